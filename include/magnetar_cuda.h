@@ -55,8 +55,11 @@ typedef enum mg_status {
 /* Element types: f32 everywhere, f16/bf16 for add-half/mul-half
  * (CudaHalfDType, src/kernels.rs:211-215). */
 /* MG_Q8_0: a packed weight (mg_buffer_upload_q8_0); only matmul's b, embedding's table,
- * mg_dequantize_q8 and downloads accept it. */
-typedef enum mg_dtype { MG_F32 = 0, MG_F16 = 1, MG_BF16 = 2, MG_Q8_0 = 3 } mg_dtype;
+ * mg_dequantize_q8 and downloads accept it.
+ * MG_Q4: a key/value store held in 4 bits (mg_kv_store_q4); only the kv-write and kv-read entries,
+ * mg_attention_packed's k and v, and downloads accept it.
+ * MG_SEQUENCES: a table of packed sequences (mg_sequences_create), read by the packed entries. */
+typedef enum mg_dtype { MG_F32 = 0, MG_F16 = 1, MG_BF16 = 2, MG_Q8_0 = 3, MG_Q4 = 4, MG_SEQUENCES = 5 } mg_dtype;
 
 typedef struct mg_device mg_device;     /* CudaKernels + its stream (src/kernels.rs:538-616) */
 typedef struct mg_buffer mg_buffer;     /* CudaDeviceBuffer / CudaHalfBuffer (src/kernels.rs:211-276) */
@@ -306,6 +309,89 @@ typedef struct mg_attention_params {
 } mg_attention_params;
 mg_status mg_attention(mg_device* d, const mg_buffer* q, const mg_buffer* k, const mg_buffer* v,
                        const mg_attention_params* params, mg_buffer** out);
+
+/* ---------------------------------------------------------------------------------- */
+/* Batches of packed sequences -- no counterpart in the reference, which serves one     */
+/* sequence per call.  The rows of several sequences lie one after another in one        */
+/* buffer, with no padding; a table names each sequence's rows.                          */
+/* ---------------------------------------------------------------------------------- */
+
+/* The table of `count` sequences.  Sequence i owns the next query_counts[i] rows of a packed
+ * query buffer, and key_counts[i] rows of a key/value buffer from row key_starts[i] on
+ * (key_counts NULL: as many as its queries; key_starts NULL: one after another).  Its query j
+ * stands at position key_counts[i] - query_counts[i] + j, so a prompt has as many keys as
+ * queries and a decode step has one query at the end of its keys.  Lengths of zero are
+ * accepted.  All rows lie below 2^31.  The counts are read before the call returns, and checked
+ * once here rather than by every call that takes the table. */
+mg_status mg_sequences_create(mg_device* d, uint64_t count, const uint64_t* query_counts, const uint64_t* key_counts,
+                              const uint64_t* key_starts, mg_buffer** out);
+/* Rewrites a table in place, in stream order: the same number of sequences, new rows.
+ * MG_CAPTURE_UNSUPPORTED during a capture, and while a captured step reads the table (its launches
+ * were sized and checked for the old rows; a captured step grows its keys by an advancing
+ * key_count instead). */
+mg_status mg_sequences_write(mg_buffer* sequences, uint64_t count, const uint64_t* query_counts,
+                             const uint64_t* key_counts, const uint64_t* key_starts);
+
+/* A key/value store held in 4 bits: `rows` rows of head_count * head_dimension values
+ * (head_dimension a multiple of 64), zero at first.  64 consecutive values of a row share a
+ * bfloat16 scale d = m / -8, m being the value of largest magnitude (the first of several); a
+ * value x is held as q = x / d rounded to the nearest whole number (ties to even, the quotient
+ * rounded to f32) within [-8, 7], and stands for q * d.  4.25 bits a value.  A block with an
+ * infinity or a NaN reads as NaN throughout.  Tiles of 64 rows; per tile and 64 columns one record
+ * of 2176 bytes: the rows' 32 bytes of quants (q + 8, value i in nibble i), then 64 scales. */
+mg_status mg_kv_store_q4(mg_device* d, uint64_t rows, uint64_t head_count, uint64_t head_dimension, mg_buffer** out);
+/* mg_kv_write accepts an MG_Q4 store, with f32, f16 or bf16 rows. */
+/* Packed kv-write: the packed rows [total queries, width] become the last query_counts[i] of each
+ * sequence's key rows in `store` (f32, f16 or bf16 as the rows, or MG_Q4 with any of them). */
+mg_status mg_kv_write_packed(mg_device* d, mg_buffer* store, const mg_buffer* rows, const mg_buffer* sequences);
+/* The values those rows stand for: [total queries, width] f32, read back from an MG_Q4 store. */
+mg_status mg_kv_read_packed(mg_device* d, const mg_buffer* store, const mg_buffer* sequences, mg_buffer** out);
+
+/* Attention of packed sequences, each over its own keys: q [total queries, heads * D]; k
+ * [rows, kv_heads * D] and v [rows, kv_heads * Dv] of q's dtype (f32, f16 or bf16), or both MG_Q4
+ * stores (Dv = D); out [total queries, heads * Dv] in q's dtype.  kv_head_count 0 = head_count;
+ * value_dimension 0 = head_dimension; window_size < 0 = none (requires causal); has_scale 0 =
+ * 1/sqrt(D).  key_count is not used (the table has it) and must be negative.  A query that sees no
+ * key gives zeros; keys outside a sequence or a mask are never weighed, whatever they hold.  Scores,
+ * maxima and sums in f32.  Dimensions up to 512. */
+mg_status mg_attention_packed(mg_device* d, const mg_buffer* q, const mg_buffer* k, const mg_buffer* v,
+                              const mg_buffer* sequences, const mg_attention_params* params, mg_buffer** out);
+
+/* rope with several axes (time, height, width of images and video; 1 to 4 of them): x [rows,
+ * head_count * head_width] (f32, f16 or bf16), positions [rows, axes] f32.  The `dimension` / 2
+ * pairs of a head are shared out by `sections` (their sum): order 0 gives each axis its pairs in
+ * one block; order 1 deals them out in turn -- pair i goes to axis i % axes while that axis, other
+ * than axis 0, has had fewer than its section, else to axis 0.  ladder 0: pair i turns at
+ * base^(-2 i / dimension); ladder 1: pair j of an axis with n pairs at base^(-j / n).  The frequency
+ * is rounded to f32 once; the angle is position * scale * frequency in f32.  pairing as mg_rope.
+ * inverse != 0 turns back (the gradient of the rotation).  out has x's dtype and may be x. */
+#define MG_ROPE_MAX_AXES 4
+typedef struct mg_rope_axes_params {
+    float base;  /* default 10000 */
+    float scale; /* default 1 */
+    uint64_t dimension;
+    uint64_t head_count;
+    int pairing; /* 0 interleaved, 1 half-split */
+    int order;
+    int ladder;
+    int inverse;
+    int axes;
+    uint64_t sections[MG_ROPE_MAX_AXES];
+} mg_rope_axes_params;
+mg_status mg_rope_axes(mg_device* d, const mg_buffer* x, const mg_buffer* positions, const mg_rope_axes_params* params,
+                       mg_buffer** out);
+
+/* Log probabilities of given tokens, with entropy and top alternatives: logits [rows, vocab] (f32,
+ * f16 or bf16), tokens [rows] f32 holding integers (NULL: none), top 0 to 64 and at most vocab,
+ * temperature finite and positive.  out [rows, 2 + 2 * top] f32: the token's log probability, the
+ * row's entropy (natural logarithms), the log probabilities of the `top` likeliest columns in
+ * falling order (equal logits: the lowest column first), then those columns.  A token that is not
+ * a column gives NaN (as does a NULL `tokens`), so rows without one may hold -1.  A logit of -inf
+ * has probability 0; a row with a NaN, an infinite maximum or no finite logit gives NaN
+ * throughout, columns included. */
+#define MG_LOGPROBS_MAX_TOP 64
+mg_status mg_token_logprobs(mg_device* d, const mg_buffer* logits, const mg_buffer* tokens, uint32_t top,
+                            float temperature, mg_buffer** out);
 
 /* ---------------------------------------------------------------------------------- */
 /* Executor -- ProviderExecutionApi over a tensor table keyed by resource id             */

@@ -15,7 +15,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libmagnetar_cuda.so")
 CSRC = os.path.join(_HERE, "csrc")
 
 MG_MAX_RANK = 8
-F32, F16, BF16, Q8_0 = 0, 1, 2, 3
+F32, F16, BF16, Q8_0, Q4, SEQUENCES = 0, 1, 2, 3, 4, 5
 PACKED_Q8_0 = 0
 ATTR_INT, ATTR_FLOAT, ATTR_BOOL, ATTR_STRING = 0, 1, 2, 3
 
@@ -57,6 +57,18 @@ class AttentionParams(ctypes.Structure):
         ("kv_head_count", ctypes.c_uint64), ("value_dimension", ctypes.c_uint64),
         ("window_size", ctypes.c_int64), ("causal", ctypes.c_int),
         ("key_count", ctypes.c_int64), ("has_scale", ctypes.c_int), ("scale", ctypes.c_float),
+    ]
+
+
+ROPE_MAX_AXES = 4
+
+
+class RopeAxesParams(ctypes.Structure):
+    _fields_ = [
+        ("base", ctypes.c_float), ("scale", ctypes.c_float), ("dimension", ctypes.c_uint64),
+        ("head_count", ctypes.c_uint64), ("pairing", ctypes.c_int), ("order", ctypes.c_int),
+        ("ladder", ctypes.c_int), ("inverse", ctypes.c_int), ("axes", ctypes.c_int),
+        ("sections", ctypes.c_uint64 * ROPE_MAX_AXES),
     ]
 
 
@@ -153,6 +165,14 @@ SIGNATURES = {
     "mg_gated_matmul": [_P, _P, _P, _P, _I, _I, _PP],
     "mg_matmul_gemv_fixed": [_I, _P, _P, _P, _P, _U64, _U64, _U64],
     "mg_attention": [_P, _P, _P, _P, ctypes.POINTER(AttentionParams), _PP],
+    "mg_sequences_create": [_P, _U64, _U64P, _U64P, _U64P, _PP],
+    "mg_sequences_write": [_P, _U64, _U64P, _U64P, _U64P],
+    "mg_kv_store_q4": [_P, _U64, _U64, _U64, _PP],
+    "mg_kv_write_packed": [_P, _P, _P, _P],
+    "mg_kv_read_packed": [_P, _P, _P, _PP],
+    "mg_attention_packed": [_P, _P, _P, _P, _P, ctypes.POINTER(AttentionParams), _PP],
+    "mg_rope_axes": [_P, _P, _P, ctypes.POINTER(RopeAxesParams), _PP],
+    "mg_token_logprobs": [_P, _P, _P, ctypes.c_uint32, _F, _PP],
     "mg_executor_create": [_P, _PP],
     "mg_executor_destroy": [_P],
     "mg_executor_write_tensor": [_P, _S, _I, _U64P, _P],

@@ -360,6 +360,114 @@ mg_status parse_rmsnorm(mg_executor* ex, const mg_invocation* inv, RmsInv* r) {
     return MG_OK;
 }
 
+// The attention attributes the reference parses, with its defaults and refusals.
+mg_status parse_attention(const Attrs& at, mg_attention_params* p) {
+    memset(p, 0, sizeof *p);
+    if (!at.integer("head_count", &p->head_count)) return fail(MG_ATTRIBUTE_UNSUPPORTED, "head_count");
+    if (!at.integer("head_dimension", &p->head_dimension)) return fail(MG_ATTRIBUTE_UNSUPPORTED, "head_dimension");
+    uint64_t v;
+    p->kv_head_count = at.integer("kv_head_count", &v) ? v : 0;
+    p->window_size = at.integer("window_size", &v) ? (int64_t)v : -1;
+    p->causal = at.boolean("causal", false);
+    const char* mk = at.string("attention_mask_kind");
+    if (mk) {
+        bool expected;
+        if (!strcmp(mk, "causal")) expected = true;
+        else if (!strcmp(mk, "bidirectional")) expected = false;
+        else return fail(MG_ATTRIBUTE_UNSUPPORTED, "attention_mask_kind '%s' is not implemented", mk);
+        if (expected != (p->causal != 0))
+            return fail(MG_ATTRIBUTE_UNSUPPORTED, "attention_mask_kind '%s' is inconsistent with causal=%s", mk,
+                        p->causal ? "true" : "false");
+    }
+    p->key_count = at.integer("key_count", &v) ? (int64_t)v : -1;
+    bool has_scale;
+    float scale = 0.0f;
+    MG_TRY(at.flt_opt("scale", &has_scale, &scale));
+    p->has_scale = has_scale;
+    p->scale = scale;
+    const mg_attribute* vd = at.find("value_head_dimension");
+    if (vd) {
+        if (vd->kind != MG_ATTR_INT || vd->int_value <= 0)
+            return fail(MG_ATTRIBUTE_UNSUPPORTED, "value_head_dimension must be a positive integer");
+        p->value_dimension = (uint64_t)vd->int_value;
+    }
+    if (at.find("value_head_stride") || at.find("latent_kv_width"))
+        return fail(MG_ATTRIBUTE_UNSUPPORTED, "latent and strided-value attention forms are not implemented");
+    return MG_OK;
+}
+
+// The attributes of rope-axes: "sections" as whole numbers joined by commas ("24,20,20"), the rest as
+// named strings, numbers and booleans.
+mg_status parse_rope_axes(const Attrs& at, mg_rope_axes_params* p) {
+    memset(p, 0, sizeof *p);
+    p->base = at.flt("base", 10000.0f);
+    p->scale = at.flt("scale", 1.0f);
+    if (!at.integer("dimension", &p->dimension)) return fail(MG_ATTRIBUTE_UNSUPPORTED, "dimension");
+    if (!at.integer("head_count", &p->head_count)) p->head_count = 1;
+    // one of two names, the first by default
+    auto either = [&](const char* name, const char* zero, const char* one, int* value) -> mg_status {
+        *value = 0;
+        const mg_attribute* a = at.find(name);
+        if (!a) return MG_OK;
+        const char* s = a->kind == MG_ATTR_STRING && a->string_value ? a->string_value : "(not a string)";
+        if (!strcmp(s, one)) *value = 1;
+        else if (strcmp(s, zero)) return fail(MG_ATTRIBUTE_UNSUPPORTED, "%s '%s' is not implemented", name, s);
+        return MG_OK;
+    };
+    MG_TRY(either("rotation_pairing", "interleaved", "half_split", &p->pairing));
+    MG_TRY(either("section_order", "blocks", "cyclic", &p->order));
+    MG_TRY(either("frequency_ladder", "shared", "per_axis", &p->ladder));
+    p->inverse = at.boolean("inverse", false);
+    const char* s = at.string("sections");
+    if (!s) return fail(MG_ATTRIBUTE_UNSUPPORTED, "sections must be a string of whole numbers joined by commas");
+    for (;; s++) {
+        if (p->axes == MG_ROPE_MAX_AXES) return fail(MG_ATTRIBUTE_UNSUPPORTED, "sections name more than %d axes", MG_ROPE_MAX_AXES);
+        uint64_t n = 0;
+        int digits = 0;
+        for (; *s >= '0' && *s <= '9' && digits < 9; s++, digits++) n = n * 10 + (uint64_t)(*s - '0');
+        if (digits == 0 || (*s && *s != ','))
+            return fail(MG_ATTRIBUTE_UNSUPPORTED, "sections must be whole numbers joined by commas");
+        p->sections[p->axes++] = n;
+        if (!*s) return MG_OK;
+    }
+}
+
+// Runs a packed kv-write of `kp` into `store`: in place when the invocation's output is its store, else
+// into a copy of the store kept under the output; a failed write leaves the rows as they were.
+mg_status kv_write_into(mg_executor* ex, const mg_invocation* inv, Buffer* store, k::KvPackedArgs& kp, mg_buffer** out) {
+    Device* d = ex->device;
+    if (!strcmp(inv->inputs[0], inv->output)) {
+        // A captured matmul may read the store through its operand form, which an in-place write
+        // inside the same step would leave stale.
+        if (ex->capturing && (store->prep || store->compact))
+            return fail(MG_CAPTURE_UNSUPPORTED, "an in-place kv-write into a weight read through its operand form cannot be captured");
+        buffer_drop_prep(store);
+        MG_TRY(k::kv_write_packed(d, kp));
+        *out = H(store);
+        return MG_OK;
+    }
+    Buffer* target = nullptr;
+    if (store->dtype == MG_Q4) {
+        MG_TRY(buffer_clone_opaque(d, store, &target));
+    } else {
+        MG_TRY(buffer_new(d, store->dtype, store->rank, store->shape, &target));
+        cudaError_t e = cudaMemcpyAsync(target->ptr, store->ptr, store->count * dtype_size(store->dtype), cudaMemcpyDeviceToDevice,
+                                        d->stream);
+        if (e != cudaSuccess) {
+            buffer_free(target);
+            return from_cuda(e, "copying the kv-write store");
+        }
+    }
+    kp.store = target->ptr;
+    const mg_status s = k::kv_write_packed(d, kp);
+    if (s != MG_OK) {
+        buffer_free(target);
+        return s;
+    }
+    *out = H(target);
+    return MG_OK;
+}
+
 mg_status dispatch(mg_executor* ex, const mg_invocation* inv, mg_buffer** out) {
     const char* name = inv->kernel;
     Attrs at{inv};
@@ -391,6 +499,13 @@ mg_status dispatch(mg_executor* ex, const mg_invocation* inv, mg_buffer** out) {
             return fail(MG_ATTRIBUTE_UNSUPPORTED, "kv-write needs a non-negative integer row_offset");
         MG_TRY(get_input(ex, inv, 0, &a));
         MG_TRY(get_input(ex, inv, 1, &b));
+        if (a->dtype == MG_Q4) {
+            k::KvPackedArgs kp;
+            uint64_t headroom;
+            MG_TRY(kv_write_q4_plan(dh, H(a), H(b), row_offset, &kp, &headroom));
+            kp.table.step = advancing_offset(ex, "row_offset", headroom);
+            return kv_write_into(ex, inv, a, kp, out);
+        }
         k::KvWriteArgs kw;
         MG_TRY(kv_write_plan(dh, H(a), H(b), row_offset, &kw));
         // An advancing row_offset writes at row_offset + offset (src/kernels.rs:2306-2310).
@@ -421,6 +536,60 @@ mg_status dispatch(mg_executor* ex, const mg_invocation* inv, mg_buffer** out) {
         *out = H(target);
         return MG_OK;
     }
+    if (!strcmp(name, "kv-write-packed")) {
+        // inputs: store, rows, sequences; in place when the output is the store, as kv-write
+        MG_TRY(get_input(ex, inv, 0, &a));
+        MG_TRY(get_input(ex, inv, 1, &b));
+        MG_TRY(get_input(ex, inv, 2, &c));
+        k::KvPackedArgs kp;
+        uint64_t headroom;
+        MG_TRY(kv_write_packed_plan(dh, H(a), H(b), H(c), &kp, &headroom));
+        // an advancing key_count moves the rows of every sequence on with its keys
+        kp.table.step = advancing_offset(ex, "key_count", headroom);
+        return kv_write_into(ex, inv, a, kp, out);
+    }
+    if (!strcmp(name, "kv-read-packed")) {
+        MG_TRY(get_input(ex, inv, 0, &a));
+        MG_TRY(get_input(ex, inv, 1, &b));
+        return mg_kv_read_packed(dh, H(a), H(b), out);
+    }
+    if (!strcmp(name, "attention-packed")) {
+        // inputs: q, k, v, sequences
+        Buffer* seqs = nullptr;
+        MG_TRY(get_input(ex, inv, 0, &a));
+        MG_TRY(get_input(ex, inv, 1, &b));
+        MG_TRY(get_input(ex, inv, 2, &c));
+        MG_TRY(get_input(ex, inv, 3, &seqs));
+        mg_attention_params p;
+        MG_TRY(parse_attention(at, &p));
+        k::PackedAttentionArgs pa;
+        uint64_t headroom;
+        MG_TRY(attention_packed_plan(dh, H(a), H(b), H(c), H(seqs), &p, out, &pa, &headroom));
+        // an advancing key_count gives every sequence as many more keys
+        pa.table.step = advancing_offset(ex, "key_count", headroom);
+        if (pa.table.step) pa.max_step = headroom;
+        return k::attention_packed(ex->device, pa);
+    }
+    if (!strcmp(name, "rope-axes")) {
+        // inputs: x, positions
+        MG_TRY(get_input(ex, inv, 0, &a));
+        MG_TRY(get_input(ex, inv, 1, &b));
+        mg_rope_axes_params p;
+        MG_TRY(parse_rope_axes(at, &p));
+        return mg_rope_axes(dh, H(a), H(b), &p, out);
+    }
+    if (!strcmp(name, "token-logprobs")) {
+        // inputs: logits, tokens (optional)
+        MG_TRY(get_input(ex, inv, 0, &a));
+        if (inv->input_count > 1) MG_TRY(get_input(ex, inv, 1, &b));
+        uint64_t top = 0;
+        const mg_attribute* ta = at.find("top");
+        if (ta && !at.integer("top", &top)) return fail(MG_ATTRIBUTE_UNSUPPORTED, "top must be a non-negative integer");
+        bool present;
+        float temperature = 1.0f;
+        MG_TRY(at.flt_opt("temperature", &present, &temperature));
+        return mg_token_logprobs(dh, H(a), b ? H(b) : nullptr, (uint32_t)std::min<uint64_t>(top, UINT32_MAX), present ? temperature : 1.0f, out);
+    }
     if (!strcmp(name, "embedding")) {
         MG_TRY(get_input(ex, inv, 0, &a));
         MG_TRY(get_input(ex, inv, 1, &b));
@@ -449,37 +618,7 @@ mg_status dispatch(mg_executor* ex, const mg_invocation* inv, mg_buffer** out) {
         MG_TRY(get_input(ex, inv, 1, &b));
         MG_TRY(get_input(ex, inv, 2, &c));
         mg_attention_params p;
-        memset(&p, 0, sizeof p);
-        if (!at.integer("head_count", &p.head_count)) return fail(MG_ATTRIBUTE_UNSUPPORTED, "head_count");
-        if (!at.integer("head_dimension", &p.head_dimension)) return fail(MG_ATTRIBUTE_UNSUPPORTED, "head_dimension");
-        uint64_t v;
-        p.kv_head_count = at.integer("kv_head_count", &v) ? v : 0;
-        p.window_size = at.integer("window_size", &v) ? (int64_t)v : -1;
-        p.causal = at.boolean("causal", false);
-        const char* mk = at.string("attention_mask_kind");
-        if (mk) {
-            bool expected;
-            if (!strcmp(mk, "causal")) expected = true;
-            else if (!strcmp(mk, "bidirectional")) expected = false;
-            else return fail(MG_ATTRIBUTE_UNSUPPORTED, "attention_mask_kind '%s' is not implemented", mk);
-            if (expected != (p.causal != 0))
-                return fail(MG_ATTRIBUTE_UNSUPPORTED, "attention_mask_kind '%s' is inconsistent with causal=%s", mk,
-                            p.causal ? "true" : "false");
-        }
-        p.key_count = at.integer("key_count", &v) ? (int64_t)v : -1;
-        bool has_scale;
-        float scale = 0.0f;
-        MG_TRY(at.flt_opt("scale", &has_scale, &scale));
-        p.has_scale = has_scale;
-        p.scale = scale;
-        const mg_attribute* vd = at.find("value_head_dimension");
-        if (vd) {
-            if (vd->kind != MG_ATTR_INT || vd->int_value <= 0)
-                return fail(MG_ATTRIBUTE_UNSUPPORTED, "value_head_dimension must be a positive integer");
-            p.value_dimension = (uint64_t)vd->int_value;
-        }
-        if (at.find("value_head_stride") || at.find("latent_kv_width"))
-            return fail(MG_ATTRIBUTE_UNSUPPORTED, "latent and strided-value attention forms are not implemented");
+        MG_TRY(parse_attention(at, &p));
         k::AttentionArgs aa;
         MG_TRY(attention_plan(dh, H(a), H(b), H(c), &p, out, &aa));
         // An advancing key_count admits key_count + offset keys (src/kernels.rs:6630-6640).
@@ -1029,6 +1168,12 @@ mg_status mg_executor_copy_tensor(mg_executor* ex, const char* from, const char*
     if (!strcmp(from, to)) return MG_OK;
     Buffer* src = it->second;
     Buffer* nb = nullptr;
+    if (opaque(src->dtype)) {
+        MG_TRY(buffer_clone_opaque(ex->device, src, &nb));
+        store_replace(ex, to, nb);
+        ex->sharded.erase(to);
+        return MG_OK;
+    }
     MG_TRY(buffer_new(ex->device, src->dtype, src->rank, src->shape, &nb));
     cudaError_t e = cudaSuccess;
     if (src->dtype == MG_Q8_0) {  // a packed weight: its layout, quants and scales
@@ -1508,6 +1653,7 @@ mg_status replay_io(mg_executor* ex, CapturedStep* st, uint64_t offset, const mg
         if (it == ex->storage.end()) return fail(MG_EXECUTION_FAILED, "no materialized data for resource %s", io[i].id);
         Buffer* b = it->second;
         if (b->dtype == MG_Q8_0) return fail(MG_DTYPE_UNSUPPORTED, "resource %s is a packed weight", io[i].id);
+        if (opaque(b->dtype)) return fail(MG_DTYPE_UNSUPPORTED, "resource %s is a %s buffer", io[i].id, dtype_name(b->dtype));
         if (io[i].bytes != b->count * dtype_size(b->dtype))
             return fail(MG_SHAPE_UNSUPPORTED, "%llu bytes do not match resource %s of shape %s",
                         (unsigned long long)io[i].bytes, io[i].id, shape_str(b).c_str());

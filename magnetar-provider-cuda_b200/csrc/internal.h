@@ -39,6 +39,8 @@ void clear_error();
     } while (0)
 
 // ---- device ----------------------------------------------------------------------------
+constexpr int kScratchSlots = 10;
+
 struct Device {
     int ordinal = 0;
     cudaStream_t own_stream = nullptr;
@@ -69,8 +71,8 @@ struct Device {
     // sets MAGNETAR_CUDA_PDL=0).
     bool pdl = true;
     // Workspaces grown on demand (see scratch()); freed in stream order.
-    void* scratch_ptr[8] = {nullptr};
-    size_t scratch_bytes[8] = {0};
+    void* scratch_ptr[kScratchSlots] = {nullptr};
+    size_t scratch_bytes[kScratchSlots] = {0};
     // Allocations made while a step capture records the stream use plain cudaMalloc (a
     // captured graph must keep addressing the same memory on every replay); frees requested
     // during a capture wait until the capture ends.
@@ -118,6 +120,23 @@ void device_free(Device* d, void* ptr);
 mg_status scratch(Device* d, int slot, size_t bytes, void** ptr);
 
 // ---- buffers -----------------------------------------------------------------------------
+// One sequence of a packed batch, as the kernels read it.
+struct SeqRow {
+    uint32_t q_start, q_count, k_start, k_count;
+};
+
+// The host side of a table of packed sequences (MG_SEQUENCES).  On the device the buffer holds the
+// rows and then the sequences' indices in falling order of their key counts.
+struct SequenceTable {
+    std::vector<SeqRow> rows;
+    uint64_t queries = 0;      // all sequences' queries
+    uint64_t key_end = 0;      // one past the last key row any sequence reads
+    uint64_t max_queries = 0;  // of one sequence
+    bool writable = true;      // no sequence has fewer keys than queries
+    // Keys every sequence may gain before one of them runs into the rows of another.
+    uint64_t slack = UINT64_MAX;
+};
+
 struct Buffer {
     Device* device = nullptr;
     mg_dtype dtype = MG_F32;
@@ -159,7 +178,19 @@ struct Buffer {
     // 4 KB record of scales ([256][4]), records ordered tile-major; stored rows padded to a
     // multiple of 256 with zeros.  Otherwise quants [q8_rows][q8_cols] and scales one per 32.
     int q8_tiled = 0;
+    // A table of packed sequences (dtype MG_SEQUENCES); null otherwise.
+    SequenceTable* seq = nullptr;
 };
+
+// A 4-bit store (dtype MG_Q4, shape [rows, width]): tiles of 64 rows, per tile and 64 columns a
+// record of 64 x 32 bytes of quants and 64 bfloat16 scales, records of a tile side by side.
+constexpr uint64_t kQ4Tile = 64;      // rows of a tile
+constexpr uint64_t kQ4Block = 64;     // values that share a scale: the columns of a record
+constexpr uint64_t kQ4Quants = 2048;  // bytes of quants in a record, in front of its scales
+constexpr uint64_t kQ4Record = kQ4Quants + 128;
+inline uint64_t q4_bytes(uint64_t rows, uint64_t width) {
+    return (rows + kQ4Tile - 1) / kQ4Tile * (width / kQ4Block) * kQ4Record;
+}
 
 // Rows a packed weight's arrays hold (padded when tiled), and the arrays' bytes.
 inline uint64_t q8_rows_held(const Buffer* b) { return b->q8_tiled ? (b->q8_rows + 255) / 256 * 256 : b->q8_rows; }
@@ -174,13 +205,24 @@ void buffer_drop_prep(Buffer* b);
 
 inline Buffer* buf(mg_buffer* b) { return reinterpret_cast<Buffer*>(b); }
 inline const Buffer* buf(const mg_buffer* b) { return reinterpret_cast<const Buffer*>(b); }
-inline size_t dtype_size(mg_dtype t) { return t == MG_F32 ? 4 : t == MG_Q8_0 ? 1 : 2; }
+// Bytes of one element; 0 for the types that have no element of their own (a 4-bit store, a table).
+inline size_t dtype_size(mg_dtype t) {
+    return t == MG_F32 ? 4 : t == MG_Q8_0 ? 1 : t == MG_Q4 || t == MG_SEQUENCES ? 0 : 2;
+}
+// The types whose contents only their own entries read and write (packed weights have rules of their own).
+inline bool opaque(mg_dtype t) { return t == MG_Q4 || t == MG_SEQUENCES; }
+// The element types of activations.
+inline bool is_float(mg_dtype t) { return t == MG_F32 || t == MG_F16 || t == MG_BF16; }
 const char* dtype_name(mg_dtype t);
 std::string shape_str(const Buffer* b);
 bool same_shape(const Buffer* a, const Buffer* b);
 
 mg_status buffer_new(Device* d, mg_dtype dtype, int rank, const uint64_t* shape, Buffer** out);
 void buffer_free(Buffer* b);
+// A buffer of `bytes` device bytes whose elements have no size of their own (opaque types).
+mg_status buffer_new_opaque(Device* d, mg_dtype dtype, int rank, const uint64_t* shape, uint64_t bytes, Buffer** out);
+// A copy of an opaque buffer, in stream order.
+mg_status buffer_clone_opaque(Device* d, const Buffer* src, Buffer** out);
 // Output-offer rule: reuse *out when it matches (dtype, element count), else allocate.
 mg_status output_for(Device* d, mg_dtype dtype, int rank, const uint64_t* shape, mg_buffer** out,
                      Buffer** result);
@@ -324,6 +366,67 @@ struct AttentionArgs {
 };
 mg_status attention(Device* d, const AttentionArgs& a);
 
+// ---- batches of packed sequences ---------------------------------------------------------
+// The table as kernels take it: `count` sequences, their order of falling key counts, and a
+// captured step's advancing key count (null: none), which every sequence's keys grow by.
+struct SeqTable {
+    const SeqRow* rows;
+    const uint32_t* order;
+    uint32_t count;
+    const uint64_t* step = nullptr;
+};
+struct KvPackedArgs {
+    const void* rows;  // packed rows [queries, width] (kv_read: the f32 output)
+    mg_dtype dtype;    // of the rows
+    void* store;
+    mg_dtype store_dtype;
+    uint64_t queries, width;
+    // Either the sequences' last rows (table.count > 0), or rows row_offset + *table.step and on.
+    SeqTable table;
+    uint64_t row_offset = 0;
+};
+mg_status kv_write_packed(Device* d, const KvPackedArgs& a);
+mg_status kv_read_packed(Device* d, const KvPackedArgs& a, float* out);
+struct PackedAttentionArgs {
+    const void *q, *k, *v;
+    void* out;
+    mg_dtype dtype;     // of q and out
+    mg_dtype kv_dtype;  // of k and v: dtype, or MG_Q4
+    uint64_t queries, kv_rows;
+    uint64_t head_count, kv_head_count, head_dim, value_dim;
+    int causal;
+    int64_t window;  // -1 none
+    float scale;
+    SeqTable table;
+    const SequenceTable* host;
+    uint64_t max_step = 0;  // the largest value *table.step takes
+};
+mg_status attention_packed(Device* d, const PackedAttentionArgs& a);
+constexpr uint64_t kPackedMaxDim = 512;
+struct RopeAxesArgs {
+    const void* x;
+    void* out;
+    const float* positions;
+    mg_dtype dtype;
+    uint64_t rows, head_count, head_width, half;
+    float scale;
+    int axes, half_split, inverse;
+    std::vector<float> frequency;  // per pair
+    std::vector<uint8_t> axis;     // per pair
+};
+constexpr uint64_t kRopeAxesMaxPairs = 512;
+mg_status rope_axes(Device* d, const RopeAxesArgs& a);
+struct LogprobsArgs {
+    const void* logits;
+    mg_dtype dtype;
+    const float* tokens;
+    float* out;
+    uint64_t rows, vocab;
+    uint32_t top;
+    float temperature;
+};
+mg_status token_logprobs(Device* d, const LogprobsArgs& a);
+
 // One launch for `count` (1-3) plain matmuls that share A and their shape (a grouped
 // projection), each optionally also written rotated by `rope` into rope_outs[i] (null: none).
 bool gemm_group_eligible(const GemmArgs* gs, int count, const RopeArgs* rope, float* const* rope_outs);
@@ -347,6 +450,18 @@ mg_status kv_write_plan(mg_device* h, mg_buffer* store, const mg_buffer* rows, u
 // attention's validation and output (launch: k::attention).
 mg_status attention_plan(mg_device* h, const mg_buffer* q, const mg_buffer* k, const mg_buffer* v,
                          const mg_attention_params* p, mg_buffer** out, k::AttentionArgs* a);
+
+// The packed entries' validation and outputs (launch: k::kv_write_packed, k::kv_read_packed,
+// k::attention_packed, k::rope_axes, k::token_logprobs).  `headroom` receives the largest number of
+// keys a captured step may add to every sequence.
+mg_status kv_write_packed_plan(mg_device* h, mg_buffer* store, const mg_buffer* rows, const mg_buffer* sequences,
+                               k::KvPackedArgs* a, uint64_t* headroom);
+mg_status attention_packed_plan(mg_device* h, const mg_buffer* q, const mg_buffer* k, const mg_buffer* v,
+                                const mg_buffer* sequences, const mg_attention_params* p, mg_buffer** out,
+                                k::PackedAttentionArgs* a, uint64_t* headroom);
+// mg_kv_write into a 4-bit store.
+mg_status kv_write_q4_plan(mg_device* h, mg_buffer* store, const mg_buffer* rows, uint64_t row_offset,
+                           k::KvPackedArgs* a, uint64_t* headroom);
 
 inline mg_status launched(Device* d, const char* what) {
     d->launches.fetch_add(1, std::memory_order_relaxed);

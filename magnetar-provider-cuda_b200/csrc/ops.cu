@@ -100,7 +100,7 @@ mg_status half_impl(mg_device* h, const mg_buffer* ah, const mg_buffer* bh, mg_b
     MG_TRY(same_device(d, a));
     MG_TRY(same_device(d, b));
     // src/kernels.rs:2227-2266: both operands share shape and half dtype.
-    if (a->dtype == MG_F32 || b->dtype == MG_F32)
+    if (a->dtype == MG_F32 || b->dtype == MG_F32 || opaque(a->dtype) || opaque(b->dtype))
         return fail(MG_DTYPE_UNSUPPORTED, "%s expects f16 or bf16 operands", op ? "mul-half" : "add-half");
     if (a->dtype != b->dtype)
         return fail(MG_DTYPE_UNSUPPORTED, "%s operands differ in dtype: %s vs %s", op ? "mul-half" : "add-half",
@@ -692,6 +692,12 @@ mg_status kv_write_plan(mg_device* h, mg_buffer* sh, const mg_buffer* rh, uint64
 extern "C" {
 
 mg_status mg_kv_write(mg_device* h, mg_buffer* store, const mg_buffer* rows, uint64_t row_offset) {
+    if (store && buf(store)->dtype == MG_Q4) {
+        k::KvPackedArgs p;
+        uint64_t headroom;
+        MG_TRY(kv_write_q4_plan(h, store, rows, row_offset, &p, &headroom));
+        return k::kv_write_packed(dev(h), p);
+    }
     k::KvWriteArgs a;
     MG_TRY(kv_write_plan(h, store, rows, row_offset, &a));
     buffer_drop_prep(buf(store));  // its contents change

@@ -50,6 +50,8 @@ const char* dtype_name(mg_dtype t) {
         case MG_F16: return "f16";
         case MG_BF16: return "bf16";
         case MG_Q8_0: return "q8_0";
+        case MG_Q4: return "q4";
+        case MG_SEQUENCES: return "sequences";
     }
     return "?";
 }
@@ -190,7 +192,7 @@ mg_status scratch(Device* d, int slot, size_t bytes, void** ptr) {
 }
 
 static void scratch_release(Device* d) {
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < kScratchSlots; i++) {
         if (d->scratch_ptr[i]) device_free(d, d->scratch_ptr[i]);
         d->scratch_ptr[i] = nullptr;
         d->scratch_bytes[i] = 0;
@@ -230,6 +232,49 @@ mg_status buffer_new(Device* d, mg_dtype dtype, int rank, const uint64_t* shape,
     return MG_OK;
 }
 
+mg_status buffer_new_opaque(Device* d, mg_dtype dtype, int rank, const uint64_t* shape, uint64_t bytes, Buffer** out) {
+    Buffer* b = new (std::nothrow) Buffer();
+    if (!b) return fail(MG_EXECUTION_FAILED, "host allocation failed");
+    b->device = d;
+    b->dtype = dtype;
+    b->rank = rank;
+    b->count = 1;
+    for (int i = 0; i < rank; i++) {
+        b->shape[i] = shape[i];
+        b->count *= shape[i];
+    }
+    mg_status s = device_alloc(d, bytes, &b->ptr);
+    if (s != MG_OK) {
+        delete b;
+        return s;
+    }
+    device_ref(d);
+    *out = b;
+    return MG_OK;
+}
+
+mg_status buffer_clone_opaque(Device* d, const Buffer* src, Buffer** out) {
+    const uint64_t bytes = src->dtype == MG_Q4 ? q4_bytes(src->shape[0], src->shape[1])
+                                               : src->seq->rows.size() * (sizeof(SeqRow) + sizeof(uint32_t));
+    Buffer* b = nullptr;
+    MG_TRY(buffer_new_opaque(d, src->dtype, src->rank, src->shape, bytes, &b));
+    if (src->seq) {
+        b->seq = new (std::nothrow) SequenceTable(*src->seq);
+        if (!b->seq) {
+            buffer_free(b);
+            return fail(MG_EXECUTION_FAILED, "host allocation failed");
+        }
+    }
+    cudaError_t e = cudaSuccess;
+    if (bytes) e = cudaMemcpyAsync(b->ptr, src->ptr, bytes, cudaMemcpyDeviceToDevice, d->stream);
+    if (e != cudaSuccess) {
+        buffer_free(b);
+        return from_cuda(e, "copying a buffer");
+    }
+    *out = b;
+    return MG_OK;
+}
+
 void buffer_drop_prep(Buffer* b) {
     if (b->prep || b->compact) b->device->prep_gen.fetch_add(1);
     if (b->prep) device_free(b->device, b->prep);
@@ -248,6 +293,7 @@ void buffer_free(Buffer* b) {
     buffer_drop_prep(b);
     if (b->owned && b->ptr) device_free(d, b->ptr);
     if (b->q8_scales) device_free(d, b->q8_scales);
+    delete b->seq;
     delete b;
     device_unref(d);
 }
@@ -480,6 +526,7 @@ mg_status mg_buffer_zeros(mg_device* h, mg_dtype dtype, int rank, const uint64_t
 mg_status mg_buffer_wrap(mg_device* h, mg_dtype dtype, int rank, const uint64_t* shape, void* ptr, mg_buffer** out) {
     if (!h || !out || (rank > 0 && !shape)) return fail(MG_INVALID_ARGUMENT, "null argument");
     MG_TRY(device_check(h));
+    if (opaque(dtype)) return fail(MG_DTYPE_UNSUPPORTED, "a %s buffer cannot be wrapped", dtype_name(dtype));
     if (rank < 0 || rank > MG_MAX_RANK) return fail(MG_SHAPE_UNSUPPORTED, "rank %d is outside 0..%d", rank, MG_MAX_RANK);
     uint64_t count;
     if (!shape_count(rank, shape, &count)) return fail(MG_SHAPE_UNSUPPORTED, "element count overflows");
@@ -509,6 +556,7 @@ mg_status mg_buffer_upload(mg_buffer* h, const void* host, uint64_t bytes) {
     if (!h || (!host && bytes)) return fail(MG_INVALID_ARGUMENT, "null argument");
     Buffer* b = buf(h);
     if (b->dtype == MG_Q8_0) return fail(MG_DTYPE_UNSUPPORTED, "a packed weight is written by mg_buffer_upload_q8_0 only");
+    if (opaque(b->dtype)) return fail(MG_DTYPE_UNSUPPORTED, "a %s buffer is written by its own entries only", dtype_name(b->dtype));
     if (bytes != b->count * dtype_size(b->dtype))
         return fail(MG_SHAPE_UNSUPPORTED, "%llu bytes cannot fill a %s buffer of shape %s",
                     (unsigned long long)bytes, dtype_name(b->dtype), shape_str(b).c_str());
@@ -523,6 +571,7 @@ mg_status mg_buffer_download(const mg_buffer* h, void* host, uint64_t bytes) {
     if (!h || (!host && bytes)) return fail(MG_INVALID_ARGUMENT, "null argument");
     const Buffer* b = buf(h);
     if (b->dtype == MG_Q8_0) return fail(MG_DTYPE_UNSUPPORTED, "a packed weight downloads as f32 values only");
+    if (opaque(b->dtype)) return fail(MG_DTYPE_UNSUPPORTED, "a %s buffer has no raw download", dtype_name(b->dtype));
     if (bytes != b->count * dtype_size(b->dtype))
         return fail(MG_SHAPE_UNSUPPORTED, "%llu bytes cannot hold a %s buffer of shape %s",
                     (unsigned long long)bytes, dtype_name(b->dtype), shape_str(b).c_str());
@@ -537,6 +586,7 @@ mg_status mg_buffer_upload_f32(mg_buffer* h, const float* host, uint64_t count) 
     if (!h || (!host && count)) return fail(MG_INVALID_ARGUMENT, "null argument");
     Buffer* b = buf(h);
     if (b->dtype == MG_Q8_0) return fail(MG_DTYPE_UNSUPPORTED, "a packed weight is written by mg_buffer_upload_q8_0 only");
+    if (opaque(b->dtype)) return fail(MG_DTYPE_UNSUPPORTED, "a %s buffer is written by its own entries only", dtype_name(b->dtype));
     if (count != b->count)
         return fail(MG_SHAPE_UNSUPPORTED, "%llu values cannot fill a buffer of shape %s",
                     (unsigned long long)count, shape_str(b).c_str());
@@ -556,6 +606,7 @@ mg_status mg_buffer_upload_f32(mg_buffer* h, const float* host, uint64_t count) 
 mg_status mg_buffer_download_f32(const mg_buffer* h, float* host, uint64_t count) {
     if (!h || (!host && count)) return fail(MG_INVALID_ARGUMENT, "null argument");
     const Buffer* b = buf(h);
+    if (b->dtype == MG_SEQUENCES) return fail(MG_DTYPE_UNSUPPORTED, "a table of sequences does not download");
     if (count != b->count)
         return fail(MG_SHAPE_UNSUPPORTED, "%llu values cannot hold a buffer of shape %s",
                     (unsigned long long)count, shape_str(b).c_str());
@@ -564,7 +615,15 @@ mg_status mg_buffer_download_f32(const mg_buffer* h, float* host, uint64_t count
     MG_CUDA(cudaSetDevice(d->ordinal), "selecting the device");
     void* staging = nullptr;
     MG_TRY(device_alloc(d, count * 4, &staging));
+    k::KvPackedArgs whole{};  // every row of a 4-bit store
+    if (b->dtype == MG_Q4) {
+        whole.store = b->ptr;
+        whole.store_dtype = MG_Q4;
+        whole.queries = b->shape[0];
+        whole.width = b->shape[1];
+    }
     mg_status s = b->dtype == MG_Q8_0 ? k::q8_dequantize(d, b, (float*)staging, false)
+                  : b->dtype == MG_Q4 ? k::kv_read_packed(d, whole, (float*)staging)
                                       : k::decode_half(d, (const uint16_t*)b->ptr, (float*)staging, count, b->dtype);
     if (s == MG_OK) {
         cudaError_t e = cudaMemcpyAsync(host, staging, count * 4, cudaMemcpyDeviceToHost, d->stream);
@@ -618,6 +677,7 @@ mg_status mg_buffer_reshape(mg_buffer* h, int rank, const uint64_t* shape) {
     if (rank < 0 || rank > MG_MAX_RANK) return fail(MG_SHAPE_UNSUPPORTED, "rank %d is outside 0..%d", rank, MG_MAX_RANK);
     Buffer* b = buf(h);
     if (b->dtype == MG_Q8_0) return fail(MG_LAYOUT_UNSUPPORTED, "a packed weight keeps its logical shape");
+    if (opaque(b->dtype)) return fail(MG_LAYOUT_UNSUPPORTED, "a %s buffer keeps its shape", dtype_name(b->dtype));
     uint64_t count;
     if (!shape_count(rank, shape, &count) || count != b->count)
         return fail(MG_SHAPE_UNSUPPORTED, "cannot reshape %s to a different element count", shape_str(b).c_str());

@@ -1,0 +1,50 @@
+// Device-side reading of a table of packed sequences and of activations in any float type.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "internal.h"
+
+namespace mg {
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+__device__ __forceinline__ SeqRow seq_load(const k::SeqTable& t, uint32_t i) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(t.rows) + i);
+    return SeqRow{v.x, v.y, v.z, v.w + (t.step ? (uint32_t)*t.step : 0u)};
+}
+
+// The sequence that owns packed query row `row` (below the table's queries): the last one that
+// starts at or before it.  Empty sequences share their start with the next one, which is later.
+__device__ __forceinline__ uint32_t seq_of_query(const k::SeqTable& t, uint32_t row) {
+    uint32_t lo = 0, hi = t.count;
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (__ldg(&t.rows[mid].q_start) <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// One dtype's kernel by a generic lambda: f(T{}).
+template <class F>
+inline mg_status by_float(mg_dtype t, F&& f) {
+    switch (t) {
+        case MG_F16: return f(__half{});
+        case MG_BF16: return f(__nv_bfloat16{});
+        default: return f(float{});
+    }
+}
+
+}  // namespace mg

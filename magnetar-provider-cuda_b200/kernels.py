@@ -15,8 +15,20 @@ import numpy as np
 from . import _native as N
 from ._native import CudaError, check
 
-_DTYPES = {"f32": N.F32, "f16": N.F16, "bf16": N.BF16, "q8_0": N.Q8_0}
+_DTYPES = {"f32": N.F32, "f16": N.F16, "bf16": N.BF16, "q8_0": N.Q8_0, "q4": N.Q4, "sequences": N.SEQUENCES}
 _DTYPE_NAMES = {v: k for k, v in _DTYPES.items()}
+
+
+def _counts(values, like=None):
+    """Whole numbers as a uint64 array (None: none); as many as ``like``."""
+    if values is None:
+        return None
+    values = [int(v) for v in values]
+    if like is not None and len(values) != len(like):
+        raise ValueError(f"{len(values)} counts for {len(like)} sequences")
+    if any(v < 0 for v in values):
+        raise ValueError("counts must not be negative")
+    return (ctypes.c_uint64 * max(1, len(values)))(*values) if values else (ctypes.c_uint64 * 0)()
 
 
 def _dtype_code(dtype) -> int:
@@ -229,6 +241,29 @@ class CudaKernels:
         dt = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}[t.dtype]
         return self.wrap(t.data_ptr(), tuple(t.shape), dt, owner=t)
 
+    # ---- batches of packed sequences ---------------------------------------------------
+    def sequences(self, query_counts, key_counts=None, key_starts=None) -> DeviceBuffer:
+        """The table of a packed batch: sequence i owns the next ``query_counts[i]`` rows of the packed
+        queries and ``key_counts[i]`` key rows (default: as many) from ``key_starts[i]`` on (default:
+        one sequence after another)."""
+        q, k, s = _counts(query_counts), _counts(key_counts, query_counts), _counts(key_starts, query_counts)
+        out = ctypes.c_void_p()
+        check(N.lib().mg_sequences_create(self._h, len(q), q, k, s, ctypes.byref(out)))
+        return DeviceBuffer(out.value, self)
+
+    def write_sequences(self, table, query_counts, key_counts=None, key_starts=None) -> DeviceBuffer:
+        """New rows for a table of as many sequences, in stream order."""
+        q, k, s = _counts(query_counts), _counts(key_counts, query_counts), _counts(key_starts, query_counts)
+        check(N.lib().mg_sequences_write(table.handle, len(q), q, k, s))
+        return table
+
+    def kv_store_q4(self, rows: int, head_count: int, head_dimension: int) -> DeviceBuffer:
+        """A key or value store of ``rows`` rows held in 4 bits (blocks of 64 values with a bfloat16
+        scale), zero at first.  ``kv_write`` and ``kv_write_packed`` write it."""
+        out = ctypes.c_void_p()
+        check(N.lib().mg_kv_store_q4(self._h, int(rows), int(head_count), int(head_dimension), ctypes.byref(out)))
+        return DeviceBuffer(out.value, self)
+
     # ---- kernels ----------------------------------------------------------------------
     def _run(self, fn, *args, out: Optional[DeviceBuffer] = None) -> DeviceBuffer:
         o = ctypes.c_void_p(out.handle.value if out is not None else None)
@@ -354,13 +389,62 @@ class CudaKernels:
     def attention(self, q, k, v, head_count, head_dimension, kv_head_count=None, window_size=None,
                   causal=False, key_count=None, scale=None, value_dimension=None, out=None):
         """``attention_valued`` (``src/kernels.rs:6505``)."""
-        p = N.AttentionParams()
-        p.head_count, p.head_dimension = head_count, head_dimension
-        p.kv_head_count = kv_head_count or 0
-        p.value_dimension = value_dimension or 0
-        p.window_size = -1 if window_size is None else int(window_size)
-        p.causal = int(bool(causal))
-        p.key_count = -1 if key_count is None else int(key_count)
-        p.has_scale = 0 if scale is None else 1
-        p.scale = 0.0 if scale is None else float(scale)
+        p = _attention_params(head_count, head_dimension, kv_head_count, window_size, causal, key_count, scale,
+                              value_dimension)
         return self._run(N.lib().mg_attention, q.handle, k.handle, v.handle, ctypes.byref(p), out=out)
+
+    def attention_packed(self, q, k, v, sequences, head_count, head_dimension, kv_head_count=None, window_size=None,
+                         causal=True, scale=None, value_dimension=None, out=None):
+        """Attention of packed sequences (``sequences``), each over its own keys; ``k`` and ``v`` have
+        ``q``'s dtype, or are 4-bit stores.  The output has ``q``'s dtype."""
+        p = _attention_params(head_count, head_dimension, kv_head_count, window_size, causal, None, scale, value_dimension)
+        return self._run(N.lib().mg_attention_packed, q.handle, k.handle, v.handle, sequences.handle, ctypes.byref(p), out=out)
+
+    def kv_write_packed(self, store, rows, sequences):
+        """Packed ``rows`` over the last ``query_counts[i]`` key rows of each sequence, in place."""
+        check(N.lib().mg_kv_write_packed(self._h, store.handle, rows.handle, sequences.handle))
+        return store
+
+    def kv_read_packed(self, store, sequences, out=None):
+        """The values of those rows of a 4-bit store, as f32."""
+        return self._run(N.lib().mg_kv_read_packed, store.handle, sequences.handle, out=out)
+
+    def rope_axes(self, x, positions, sections, base=10000.0, scale=1.0, dimension=None, head_count=1,
+                  pairing="interleaved", order="blocks", ladder="shared", inverse=False, out=None):
+        """Rotary positions with several axes: ``positions`` [rows, axes], ``sections`` the pairs of each
+        axis, in one block each (``order="blocks"``) or dealt out in turn (``"cyclic"``), over one set
+        of frequencies (``ladder="shared"``) or one per axis (``"per_axis"``).  ``inverse`` turns back,
+        which is also the rotation's gradient.  ``out`` may be ``x``."""
+        p = N.RopeAxesParams()
+        p.base, p.scale = base, scale
+        p.dimension = dimension if dimension is not None else x.shape[-1] // max(1, head_count)
+        p.head_count = head_count
+        p.pairing = {"interleaved": 0, "half_split": 1}[pairing]
+        p.order = {"blocks": 0, "cyclic": 1}[order]
+        p.ladder = {"shared": 0, "per_axis": 1}[ladder]
+        p.inverse = int(bool(inverse))
+        sections = [int(s) for s in sections]
+        if not 1 <= len(sections) <= N.ROPE_MAX_AXES or min(sections) < 0:
+            raise CudaError(1, f"RoPE takes 1 to {N.ROPE_MAX_AXES} axes with sections that are not negative, got {sections}")
+        p.axes = len(sections)
+        p.sections[:len(sections)] = sections
+        return self._run(N.lib().mg_rope_axes, x.handle, positions.handle, ctypes.byref(p), out=out)
+
+    def token_logprobs(self, logits, tokens=None, top=0, temperature=1.0, out=None):
+        """[rows, 2 + 2 * top]: the log probability of each row's token (NaN without one), the row's
+        entropy, the log probabilities of the ``top`` likeliest columns, and those columns."""
+        return self._run(N.lib().mg_token_logprobs, logits.handle, tokens.handle if tokens is not None else None,
+                         int(top), ctypes.c_float(temperature), out=out)
+
+
+def _attention_params(head_count, head_dimension, kv_head_count, window_size, causal, key_count, scale, value_dimension):
+    p = N.AttentionParams()
+    p.head_count, p.head_dimension = head_count, head_dimension
+    p.kv_head_count = kv_head_count or 0
+    p.value_dimension = value_dimension or 0
+    p.window_size = -1 if window_size is None else int(window_size)
+    p.causal = int(bool(causal))
+    p.key_count = -1 if key_count is None else int(key_count)
+    p.has_scale = 0 if scale is None else 1
+    p.scale = 0.0 if scale is None else float(scale)
+    return p

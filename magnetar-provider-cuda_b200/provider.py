@@ -53,6 +53,12 @@ def _half(base, family, device, provider):
                                device=device, input_dtypes=("f16", "bf16"), output_dtypes=("f16", "bf16"))
 
 
+def _batch(name, family, device, provider, features=(), outputs=("f32", "f16", "bf16")):
+    # f32, f16 or bf16 activations in rank-2 packed buffers
+    return KernelAdvertisement(name=name, operator=name, family=family, provider=provider, device=device,
+                               input_dtypes=("f32", "f16", "bf16"), output_dtypes=outputs, rank=2, features=tuple(features))
+
+
 def cuda_kernel_advertisements(device: str, provider: str = CUDA_PROVIDER_NAME) -> List[KernelAdvertisement]:
     """The implemented kernel set for one device (``cuda_kernel_advertisements``)."""
     return [
@@ -78,6 +84,12 @@ def cuda_kernel_advertisements(device: str, provider: str = CUDA_PROVIDER_NAME) 
         _baseline("concat", "Tensor", device, provider, ["heads"]),  # rows, or heads (axis = "heads")
         _baseline("batched-matmul", "LinearAlgebra", device, provider),
         _baseline("kv-write", "Tensor", device, provider),  # f32 stores, in place
+        # batches of packed sequences (no counterpart in the reference's registry)
+        _batch("attention-packed", "Attention", device, provider, ["attention-q4-store", "attention-scale", "attention-window"]),
+        _batch("kv-write-packed", "Tensor", device, provider, ["q4-store"]),
+        _batch("kv-read-packed", "Tensor", device, provider, ["q4-store"], outputs=("f32",)),
+        _batch("rope-axes", "PositionEncoding", device, provider, ["rope-inverse"]),
+        _batch("token-logprobs", "Activation", device, provider, ["entropy", "top"], outputs=("f32",)),
         _half("add", "Tensor", device, provider),
         _half("mul", "Tensor", device, provider),
     ]
