@@ -1,0 +1,724 @@
+// Attention of packed sequences on the 5th-generation tensor cores: head dimensions 64 and 128, f32,
+// bfloat16 and f16.
+//
+// A CTA serves 256 query rows of one sequence as two 128-row tiles that share every tile of keys and
+// values it loads.  A row is one (token, head): where the heads that share a key/value head are a
+// multiple of a power of two, that many heads of a token are neighbouring rows (grouped heads read
+// each key once, and short prompts fill their tiles).  Warp 0 loads with TMA, warp 1 issues the MMAs,
+// warps 2 and 3 look after the values of tiles that are not wholly visible, warps 4-7 (tile 0) and
+// 8-11 (tile 1) run the softmax, one row per thread.  While one tile's softmax runs, the tensor cores
+// have the other tile's products.
+//
+// S = Q K^T goes to tensor memory; the softmax writes its weights P as 16-bit values over the scores it
+// has read, and O += P V reads P from there.  The weights are 2^(s - m - offset) with a reference m that
+// moves only when a tile's maximum passes it by more than 2^kLazy; O and the sum are then rescaled.
+// The offset (2^40 for weights with f32's exponent range) keeps O below the largest |v|
+// however many keys are summed, so large finite values cannot overflow the sum.
+//
+// f32 operands are two bfloat16 terms each, hi + lo, and three products: lo hi + hi lo + hi hi; K and V
+// are split by a pass of their own into a workspace of the sequences' rows one after another, a query
+// row by the thread that owns it.
+//
+// Masks: scores of keys a row must not see become -inf.  A weight of zero does not keep out a NaN or an
+// infinity in V, though, so in tiles that some row sees only in part the value rows that no row sees
+// are zeroed in shared memory, and if a remaining one is not finite the CTA's rows are computed again
+// one by one at the end.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
+#include <type_traits>
+
+#include "attention_packed.cuh"
+#include "sm100.cuh"
+
+namespace mg {
+namespace {
+
+using namespace sm100;
+
+constexpr int kRows = 128;      // rows of a query tile (MMA M)
+constexpr int kThreads = 384;   // 12 warps
+
+template <typename T, int D>
+struct Shape {
+    static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
+    static constexpr int kKeys = kTerms == 2 ? 64 : 128;   // keys of a tile
+    static constexpr int kScores = 128 / kKeys;            // score buffers of a query tile
+    static constexpr int kQAtom = kRows * 128;             // [128 rows][64 columns], 128-byte swizzle
+    static constexpr int kQTerm = (D / 64) * kQAtom;
+    static constexpr int kQTile = kTerms * kQTerm;
+    static constexpr int kAtom = kKeys * 128;              // [keys][64 columns]
+    static constexpr int kTerm = (D / 64) * kAtom;
+    static constexpr int kStage = kTerms * kTerm;          // one tile of K, or of V
+    static constexpr int kKStages = 2;
+    static constexpr int kVStages = kTerms == 2 && D == 128 ? 1 : 2;
+    static constexpr int kOffK = 2 * kQTile;
+    static constexpr int kOffV = kOffK + kKStages * kStage;
+    static constexpr int kSmem = kOffV + kVStages * kStage + 1024;
+    static constexpr uint32_t kColO = 256;                 // tensor memory: scores of tile t at 128 t, O at 256 + D t
+};
+
+struct Params {
+    k::PackedAttentionArgs a;
+    uint32_t pack, pack_log2;   // heads of a token that are neighbouring rows (a power of two)
+    uint32_t groups;            // sets of `pack` heads
+    uint32_t tokens;            // of a CTA: 256 / pack
+    float scale2;               // scores to log2 units
+    int* error;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Two values as a packed pair of the 16-bit type, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+
+// x as two bfloat16 terms; a finite value that would round to infinity is cut instead.
+__device__ __forceinline__ void split(float x, uint16_t& hi, uint16_t& lo) {
+    __nv_bfloat16 h = __float2bfloat16_rn(x);
+    if (isinf(__bfloat162float(h)) && !isinf(x)) h = __ushort_as_bfloat16((uint16_t)(__float_as_uint(x) >> 16));
+    hi = __bfloat16_as_ushort(h);
+    lo = __bfloat16_as_ushort(__float2bfloat16_rn(x - __bfloat162float(h)));
+}
+
+// The sequences' f32 rows, one sequence after another, as their two terms.  Streaming: 4 bytes read and
+// 4 written per value.
+__global__ void __launch_bounds__(256) split_rows_kernel(k::SeqTable t, const float* __restrict__ src, uint16_t* __restrict__ hi,
+                                                         uint16_t* __restrict__ lo, uint64_t keys, uint32_t vecs) {
+    pdl_enter();
+    const uint64_t step = t.step ? *t.step : 0;
+    const uint64_t n = (keys + step * t.count) * vecs, stride = (uint64_t)gridDim.x * blockDim.x;
+    for (uint64_t w = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; w < n; w += stride) {
+        const uint32_t g = (uint32_t)(w / vecs), c = (uint32_t)(w % vecs);
+        uint32_t a = 0, b = t.count;  // the last sequence whose keys start at or before g
+        while (b - a > 1) {
+            const uint32_t mid = (a + b) / 2;
+            if (__ldg(t.key_prefix + mid) + (uint32_t)step * mid <= g) a = mid;
+            else b = mid;
+        }
+        const uint64_t row = (uint64_t)__ldg(&t.rows[a].k_start) + (g - (__ldg(t.key_prefix + a) + (uint32_t)step * a));
+        const float4 x = reinterpret_cast<const float4*>(src)[row * vecs + c];
+        uint16_t h[4], l[4];
+        split(x.x, h[0], l[0]);
+        split(x.y, h[1], l[1]);
+        split(x.z, h[2], l[2]);
+        split(x.w, h[3], l[3]);
+        reinterpret_cast<uint2*>(hi)[w] = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+        reinterpret_cast<uint2*>(lo)[w] = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
+    }
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+// Descriptor of a 16-bit operand whose rows (128 bytes, 64 consecutive values of the N dimension) are
+// the contraction: 8-row groups 1024 bytes apart, the next 64 of N `next` bytes further.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t next) {
+    uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)((next >> 4) & 0x3FFFu) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// kind::f16 with an f32 accumulator: operand format 0 f16, 1 bfloat16; B with N along its rows.
+constexpr uint32_t idesc(int format, int m, int n, bool b_mn) {
+    return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(m >> 4) << 24);
+}
+
+template <typename T, int D>
+__device__ __noinline__ void recompute_rows(const Params& p, const SeqRow& s, uint32_t tok0, uint32_t head0) {
+    const int lane = threadIdx.x % 32;
+    const uint64_t w = p.a.kv_head_count * D;
+    const PlainRows<T> kr{(const T*)p.a.k, w}, vr{(const T*)p.a.v, w};
+    for (uint32_t r = threadIdx.x / 32; r < 2 * kRows; r += kThreads / 32) {
+        const uint32_t tok = tok0 + (r >> p.pack_log2);
+        if (tok >= s.q_count) break;
+        attention_row<T, PlainRows<T>, D / 32>(p.a, kr, vr, s, s.q_start + tok, head0 + (r & (p.pack - 1)), lane);
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                               const __grid_constant__ CUtensorMap map_klo, const __grid_constant__ CUtensorMap map_v,
+                               const __grid_constant__ CUtensorMap map_vlo, const __grid_constant__ Params p) {
+    using S = Shape<T, D>;
+    constexpr int KV = S::kKeys;
+    constexpr bool kTwo = S::kTerms == 2;
+    constexpr int kFormat = std::is_same<T, __half>::value ? 0 : 1;
+    // f16 weights have no exponents to spare: they may reach 2^15, and vanish below 2^-24
+    constexpr float kLazy = kFormat == 0 ? 7.0f : 8.0f;
+    constexpr float kOffset = kFormat == 0 ? -8.0f : 40.0f;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint64_t bars[24];
+    __shared__ uint32_t tmem_slot;
+    __shared__ uint32_t s_seq, s_place, s_poison;
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - raw);
+    const uint32_t b0 = smem_u32(bars);
+    const uint32_t q_full = b0;
+    auto k_full = [&](int s) { return b0 + 8 + 8u * (uint32_t)s; };
+    auto k_empty = [&](int s) { return b0 + 24 + 8u * (uint32_t)s; };
+    auto v_full = [&](int s) { return b0 + 40 + 8u * (uint32_t)s; };
+    auto v_ready = [&](int s) { return b0 + 56 + 8u * (uint32_t)s; };
+    auto v_empty = [&](int s) { return b0 + 72 + 8u * (uint32_t)s; };
+    auto s_full = [&](int t, int b) { return b0 + 88 + 8u * (uint32_t)(2 * t + b); };
+    auto p_full = [&](int t, int b) { return b0 + 120 + 8u * (uint32_t)(2 * t + b); };
+    auto pv_done = [&](int t, int b) { return b0 + 152 + 8u * (uint32_t)(2 * t + b); };
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 23; i++) {
+            const uint32_t bar = b0 + 8u * (uint32_t)i;
+            // P: the tile's four softmax warps; Q: all eight where they split it; V: its two warps
+            const bool is_p = bar >= p_full(0, 0) && bar <= p_full(1, 1), is_v = bar >= v_ready(0) && bar <= v_ready(1);
+            mbar_init(bar, is_p ? 4 : is_v ? 2 : bar == q_full && kTwo ? 8 : 1);
+        }
+        s_poison = 0;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_slot), 512);
+        tmem_relinquish();
+    }
+    if (warp == 0) {
+        // Sequences with the most keys first, and a sequence's last (heaviest) tokens first: CTAs start in
+        // grid order, so light ones fill the last wave.  (The table was written by copies, which a
+        // launch never overtakes.)
+        uint32_t seq, place;
+        auto tiles = [&](uint32_t i) { return (__ldg(&p.a.table.rows[i].q_count) + p.tokens - 1) / p.tokens; };
+        const bool found = find_item(p.a.table, blockIdx.x / p.groups, tiles, seq, place);
+        if (lane == 0) {
+            s_seq = found ? seq : 0xffffffffu;
+            s_place = found ? tiles(seq) - 1 - place : 0;
+        }
+    }
+    pdl_enter();  // after the TMEM allocation, as every tensor-memory kernel here does
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    const bool any = s_seq != 0xffffffffu;
+    const SeqRow seq = any ? seq_load(p.a.table, s_seq) : SeqRow{0, 0, 0, 0};
+    const uint32_t tok0 = s_place * p.tokens, head0 = (blockIdx.x % p.groups) * p.pack;
+    const int kvh = (int)(head0 / (uint32_t)(p.a.head_count / p.a.kv_head_count));
+    const int m_keys = (int)seq.k_count, shift = m_keys - (int)seq.q_count;  // token i stands at shift + i
+    const int window = p.a.window >= 0 && p.a.window < 0x7fffffff ? (int)p.a.window : -1;
+    // first row of K and V: f32 terms lie in the workspace, packed
+    const int key_row0 = kTwo ? (any ? (int)(__ldg(p.a.table.key_prefix + s_seq) + (p.a.table.step ? (uint32_t)*p.a.table.step * s_seq : 0u)) : 0)
+                              : (int)seq.k_start;
+    // Keys [kv0, ...) the CTA reads, and the tiles of them each query tile reads.
+    const int live_tokens = min((int)p.tokens, (int)seq.q_count - (int)tok0);
+    const int kv0 = window > 0 ? max(0, shift + (int)tok0 - window + 1) : 0;
+    int n_t[2], hi_cta = 0;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int first = t * (int)p.tokens / 2;  // (a tile holds whole tokens: pack <= 128)
+        const int last = min(live_tokens, first + (int)p.tokens / 2) - 1;
+        const int hi = last < first ? 0 : p.a.causal ? min(m_keys, shift + (int)tok0 + last + 1) : m_keys;
+        n_t[t] = hi > kv0 ? (hi - kv0 + KV - 1) / KV : 0;
+        hi_cta = max(hi_cta, hi);
+    }
+    const int n_kv = max(n_t[0], n_t[1]);
+    // Keys every row of the CTA sees.
+    const int all_lo = window > 0 ? max(0, shift + (int)tok0 + live_tokens - window) : 0;
+    const int all_hi = p.a.causal ? min(m_keys, shift + (int)tok0 + 1) : m_keys;
+
+    if (warp == 0) {
+        // ---- TMA producer ----------------------------------------------------------------------
+        if (lane == 0 && n_kv > 0) {
+            if constexpr (!kTwo) {
+                mbar_arrive_expect_tx(q_full, 2 * S::kQTile);
+                for (int t = 0; t < 2; t++)
+                    for (int a = 0; a < D / 64; a++)
+                        tma_load_3d(base + t * S::kQTile + a * S::kQAtom, &map_q, q_full, a * 64, (int)head0,
+                                    (int)(seq.q_start + tok0) + t * (int)p.tokens / 2);
+            }
+            auto load = [&](uint32_t slot, uint32_t bar, const CUtensorMap* hi, const CUtensorMap* lo, int j) {
+                mbar_arrive_expect_tx(bar, S::kStage);
+                for (int a = 0; a < D / 64; a++) {
+                    const int x = kvh * D + a * 64, y = key_row0 + kv0 + j * KV;
+                    tma_load_2d(slot + a * S::kAtom, hi, bar, x, y);
+                    if constexpr (kTwo) tma_load_2d(slot + S::kTerm + a * S::kAtom, lo, bar, x, y);
+                }
+            };
+            auto load_k = [&](int j) -> bool {
+                const int s = j % S::kKStages;
+                if (j >= S::kKStages && !mbar_wait(k_empty(s), (uint32_t)(j / S::kKStages - 1) & 1u)) return false;
+                load(base + S::kOffK + s * S::kStage, k_full(s), &map_k, &map_klo, j);
+                return true;
+            };
+            bool ok = load_k(0);
+            for (int j = 0; j < n_kv && ok; j++) {
+                if (j + 1 < n_kv) ok = load_k(j + 1);
+                const int s = j % S::kVStages;
+                if (ok && j >= S::kVStages) ok = mbar_wait(v_empty(s), (uint32_t)(j / S::kVStages - 1) & 1u);
+                if (ok) load(base + S::kOffV + s * S::kStage, v_full(s), &map_v, &map_vlo, j);
+            }
+            if (!ok) atomicExch(p.error, 1);
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---- MMA issuer --------------------------------------------------------------------------
+        if (lane == 0 && n_kv > 0) {
+            constexpr uint32_t idesc_s = idesc(kFormat, kRows, KV, false);
+            constexpr uint32_t idesc_o = idesc(kFormat, kRows, D, true);
+            const uint64_t dq0 = desc_k_sw128(base), dk0 = desc_k_sw128(base + S::kOffK);
+            const uint64_t dv0 = desc_mn_sw128(base + S::kOffV, S::kAtom);
+            // S_t(j) = Q_t K(j)^T into tile t's score buffer j % kScores
+            auto issue_s = [&](int t, int j) {
+                const uint32_t tS = tmem + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
+                const uint64_t dq = dq0 + (uint64_t)((t * S::kQTile) >> 4);
+                const uint64_t dk = dk0 + (uint64_t)(((j % S::kKStages) * S::kStage) >> 4);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; kk++) {
+                    const uint64_t q = dq + (uint64_t)(((kk / 4) * S::kQAtom + (kk % 4) * 32) >> 4);
+                    const uint64_t k = dk + (uint64_t)(((kk / 4) * S::kAtom + (kk % 4) * 32) >> 4);
+                    if constexpr (kTwo) {
+                        mma_bf16(tS, q + (uint64_t)(S::kQTerm >> 4), k, idesc_s, kk > 0 ? 1u : 0u);
+                        mma_bf16(tS, q, k + (uint64_t)(S::kTerm >> 4), idesc_s, 1u);
+                        mma_bf16(tS, q, k, idesc_s, 1u);
+                    } else {
+                        mma_bf16(tS, q, k, idesc_s, kk > 0 ? 1u : 0u);
+                    }
+                }
+                tc_commit(s_full(t, j % S::kScores));
+            };
+            bool ok = mbar_wait(q_full, 0);
+            for (int j = 0; j < min(S::kScores, n_kv) && ok; j++) {
+                ok = mbar_wait(k_full(j), 0);
+                if (!ok) break;
+                tc_fence_after();
+                for (int t = 0; t < 2; t++)
+                    if (j < n_t[t]) issue_s(t, j);
+                tc_commit(k_empty(j));
+            }
+            for (int j = 0; j < n_kv && ok; j++) {
+                const int vs = j % S::kVStages, jn = j + S::kScores;
+                const uint32_t vp = (uint32_t)(j / S::kVStages) & 1u;
+                ok = mbar_wait(v_full(vs), vp) && mbar_wait(v_ready(vs), vp);
+                if (!ok) break;
+                tc_fence_after();
+                bool k_ready = false;
+                for (int t = 0; t < 2 && ok; t++) {
+                    if (j < n_t[t]) {
+                        ok = mbar_wait(p_full(t, j % S::kScores), (uint32_t)(j / S::kScores) & 1u);
+                        if (!ok) break;
+                        tc_fence_after();
+                        // O_t += P_t(j) V(j): P from tensor memory, two values per column
+                        const uint32_t tP = tmem + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
+                        const uint32_t tO = tmem + S::kColO + (uint32_t)(D * t);
+                        const uint64_t dv = dv0 + (uint64_t)((vs * S::kStage) >> 4);
+#pragma unroll
+                        for (int kk = 0; kk < KV / 16; kk++) {
+                            const uint64_t v = dv + (uint64_t)((kk * 2048) >> 4);
+                            const uint32_t pa = tP + (uint32_t)kk * 8;
+                            const uint32_t acc = (j > 0 || kk > 0) ? 1u : 0u;
+                            if constexpr (kTwo) {
+                                mma_bf16_ts(tO, pa + KV / 2, v, idesc_o, acc);
+                                mma_bf16_ts(tO, pa, v + (uint64_t)(S::kTerm >> 4), idesc_o, 1u);
+                                mma_bf16_ts(tO, pa, v, idesc_o, 1u);
+                            } else {
+                                mma_bf16_ts(tO, pa, v, idesc_o, acc);
+                            }
+                        }
+                        tc_commit(pv_done(t, j & 1));
+                    }
+                    if (t == 1) tc_commit(v_empty(vs));
+                    if (jn < n_t[t]) {
+                        if (!k_ready) {
+                            ok = mbar_wait(k_full(jn % S::kKStages), (uint32_t)(jn / S::kKStages) & 1u);
+                            if (!ok) break;
+                            tc_fence_after();
+                            k_ready = true;
+                        }
+                        issue_s(t, jn);
+                    }
+                }
+                if (ok && jn < n_kv) tc_commit(k_empty(jn % S::kKStages));
+            }
+            if (!ok) atomicExch(p.error, 1);
+        }
+        __syncwarp();
+    } else if (warp < 4) {
+        // ---- values of tiles some row sees only in part ------------------------------------------
+        const int i0 = (int)threadIdx.x - 64;
+        constexpr uint32_t kExponents = kFormat == 0 ? 0x7c00u : 0x7f80u;
+        bool failed = false;
+        for (int j = 0; j < n_kv && !failed; j++) {
+            const int s = j % S::kVStages;
+            failed = !mbar_wait(v_full(s), (uint32_t)(j / S::kVStages) & 1u);
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+            const int key0 = kv0 + j * KV;
+            if (key0 < all_lo || key0 + KV > all_hi) {
+                uint8_t* stage = base_ptr + S::kOffV + s * S::kStage;
+                bool bad = false;
+                for (int r = i0; r < KV; r += 64) {
+                    const bool seen = key0 + r < hi_cta;
+                    for (int a = 0; a < S::kTerms * (D / 64); a++) {
+                        uint4* row = reinterpret_cast<uint4*>(stage + a * S::kAtom + r * 128);
+#pragma unroll
+                        for (int c = 0; c < 8; c++) {
+                            uint4& v = row[(c + lane) & 7];  // (neighbouring lanes in different banks)
+                            if (!seen) {
+                                v = make_uint4(0u, 0u, 0u, 0u);
+                            } else {
+                                const uint4 x = v;
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const uint32_t u = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
+                                    bad = bad || (u & kExponents) == kExponents || ((u >> 16) & kExponents) == kExponents;
+                                }
+                            }
+                        }
+                    }
+                }
+                if (bad) s_poison = 1;
+                fence_proxy_async();  // the zeros are read by tcgen05.mma
+            }
+            mbar_arrive_warp(v_ready(s));
+        }
+        if (failed && lane == 0) atomicExch(p.error, 1);
+    } else {
+        // ---- softmax: one query row per thread ---------------------------------------------------
+        const float kNegInf = __int_as_float(0xff800000);
+        const int t = (warp - 4) / 4, qq = warp % 4;
+        const int r = qq * 32 + lane;
+        const int tile_tok0 = (int)tok0 + t * (int)p.tokens / 2;
+        const int tok = tile_tok0 + (r >> p.pack_log2);
+        const bool live = tok < (int)seq.q_count;
+        // element offset of row i of this warp in q and out
+        auto row_at = [&](int i) {
+            const int rr = qq * 32 + i;
+            const uint64_t token = (uint64_t)seq.q_start + (uint64_t)(tile_tok0 + (rr >> p.pack_log2));
+            return (token * p.a.head_count + head0 + (uint32_t)(rr & (int)(p.pack - 1))) * D;
+        };
+        auto row_live = [&](int i) { return tile_tok0 + ((qq * 32 + i) >> p.pack_log2) < (int)seq.q_count; };
+        if constexpr (kTwo) {
+            if (n_kv > 0) {
+                // This warp's 32 query rows as two terms in the MMA's K-major layout: 16-byte chunk c of a row
+                // at position c ^ (row % 8); zeros for rows past the sequence.  One row per load, each
+                // lane D / 32 columns, all rows in flight before the first is split.
+                constexpr int V = D / 32;
+                using Vec = typename std::conditional<V == 4, float4, float2>::type;
+                const float* q = (const float*)p.a.q;
+                Vec xv[32];
+#pragma unroll
+                for (int i = 0; i < 32; i++) xv[i] = row_live(i) ? __ldg(reinterpret_cast<const Vec*>(q + row_at(i) + lane * V)) : Vec{};
+                uint8_t* qt = base_ptr + t * S::kQTile;
+                const int e0 = lane * V, a = e0 / 64, c = (e0 % 64) / 8, byte = (e0 % 8) * 2;
+#pragma unroll
+                for (int i = 0; i < 32; i++) {
+                    const int rr = qq * 32 + i;
+                    const int off = a * S::kQAtom + rr * 128 + ((c ^ (rr & 7)) * 16 + byte);
+                    const float* xs = reinterpret_cast<const float*>(&xv[i]);
+                    uint16_t h[V], l[V];
+#pragma unroll
+                    for (int e = 0; e < V; e++) split(xs[e], h[e], l[e]);
+#pragma unroll
+                    for (int e = 0; e < V; e += 2) {
+                        *reinterpret_cast<uint32_t*>(qt + off + 2 * e) = h[e] | (uint32_t)h[e + 1] << 16;
+                        *reinterpret_cast<uint32_t*>(qt + S::kQTerm + off + 2 * e) = l[e] | (uint32_t)l[e + 1] << 16;
+                    }
+                }
+                fence_proxy_async();  // the generic-proxy writes are read by tcgen05.mma
+                mbar_arrive_warp(q_full);
+            }
+        }
+        // Keys [row_lo, row_hi) this row sees.
+        const int pos = shift + tok;
+        const int row_hi = !live ? 0 : p.a.causal ? max(0, min(m_keys, pos + 1)) : m_keys;
+        const int row_lo = window > 0 ? min(max(0, pos - window + 1), row_hi) : 0;
+        const float sc = p.scale2;
+        const uint32_t lane_base = tmem + ((uint32_t)(qq * 32) << 16);
+        const uint32_t tO = lane_base + S::kColO + (uint32_t)(D * t);
+        const int n = n_t[t];
+        float m = kNegInf, l = 0.0f;
+        bool failed = false;
+        for (int j = 0; j < n; j++) {
+            failed = !mbar_wait(s_full(t, j % S::kScores), (uint32_t)(j / S::kScores) & 1u);
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+            tc_fence_after();
+            const uint32_t tS = lane_base + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
+            float s[KV];
+#pragma unroll
+            for (int c = 0; c < KV; c += 32) tmem_ld32(tS + (uint32_t)c, s + c);
+            tc_wait_ld();
+            const int key0 = kv0 + j * KV;
+            if (key0 < row_lo || key0 + KV > row_hi) {
+                const int lo = row_lo - key0, hi = row_hi - key0;
+#pragma unroll
+                for (int c = 0; c < KV; c++) s[c] = c >= lo && c < hi ? s[c] : kNegInf;
+            }
+            // the row's maximum of the raw scores (sc > 0 keeps their order), in log2 units
+            float mx[4];
+#pragma unroll
+            for (int g = 0; g < 4; g++) mx[g] = fmaxf(s[g], s[g + 4]);
+#pragma unroll
+            for (int c = 8; c < KV; c += 8)
+#pragma unroll
+                for (int g = 0; g < 4; g++) mx[g] = max3(mx[g], s[c + g], s[c + 4 + g]);
+            const float tmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sc;
+            // the reference moves only when this tile's maximum passes it by more than kLazy
+            bool move = tmax != kNegInf && (m == kNegInf || tmax > m + kLazy);
+            float f = 1.0f;
+            if (move) {
+                f = m == kNegInf ? 0.0f : ex2(m - tmax);
+                move = m != kNegInf;  // an O that holds only zero weights needs no rescale
+                m = tmax;
+                l *= f;
+            }
+            // (no key seen yet: every score is -inf, and weights 2^(-inf) are 0)
+            const float ref = m == kNegInf ? 0.0f : -(m + kOffset);
+            const uint64_t sc2 = f2(sc, sc), ref2 = f2(ref, ref);
+            float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < KV; c += 2) {
+                uint64_t x = ref2;
+                f2fma(x, f2(s[c], s[c + 1]), sc2);
+                const float2 e = f2split(x);
+                s[c] = ex2(e.x);
+                s[c + 1] = ex2(e.y);
+                ps[c & 2] += s[c];
+                ps[(c & 2) + 1] += s[c + 1];
+            }
+            l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+            if (j > 0 && __any_sync(0xffffffffu, move)) {
+                // O *= f, once P V(j - 1) has completed
+                failed = !mbar_wait(pv_done(t, (j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u);
+                failed = __any_sync(0xffffffffu, failed);
+                if (failed) break;
+                tc_fence_after();
+                const float g = move ? f : 1.0f;
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                    float o[16];
+                    tmem_ld16(tO + (uint32_t)c, o);
+                    tc_wait_ld();
+                    uint32_t u[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) u[e] = __float_as_uint(o[e] * g);
+                    tmem_st16(tO + (uint32_t)c, u);
+                }
+                tc_wait_st();
+            }
+            // P over the scores just read
+#pragma unroll
+            for (int c = 0; c < KV; c += 32) {
+                uint32_t h[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) h[e] = pack16<T>(s[c + 2 * e], s[c + 2 * e + 1]);
+                tmem_st16(tS + (uint32_t)(c / 2), h);
+                if constexpr (kTwo) {
+                    uint32_t lo[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        lo[e] = pack16<T>(s[c + 2 * e] - __uint_as_float(h[e] << 16), s[c + 2 * e + 1] - __uint_as_float(h[e] & 0xffff0000u));
+                    tmem_st16(tS + (uint32_t)(KV / 2 + c / 2), lo);
+                }
+            }
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive_warp(p_full(t, j % S::kScores));
+        }
+        // ---- the output row: O / l ---------------------------------------------------------------
+        bool have = false;
+        if (n > 0 && !failed) {
+            failed = !mbar_wait(pv_done(t, (n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u);
+            failed = __any_sync(0xffffffffu, failed);
+            have = !failed;
+        }
+        if (failed) atomicExch(p.error, 1);
+        T* out = (T*)p.a.out;
+        constexpr int kChunks = D * (int)sizeof(T) / 16;  // 16-byte chunks per row
+        constexpr int kRowsPerStore = 32 / kChunks;       // rows one warp store covers
+        constexpr int N = 16 / (int)sizeof(T);
+        if (have) {
+            // Each thread writes its row into its warp's staging area -- this tile's queries, which no MMA
+            // reads once the last P V has completed -- with chunk k of row i at position k ^ i; then the
+            // warp stores whole rows, 16 bytes per lane.
+            tc_fence_after();
+            const float inv = l > 0.0f ? 1.0f / l : l != l ? l : 0.0f;
+            uint8_t* stage = base_ptr + t * S::kQTile + qq * (32 * D * (int)sizeof(T));
+            fence_proxy_async();  // after the MMAs' reads of this area, before generic writes
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
+                tmem_ld32(tO + (uint32_t)c, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; e += N) {
+                    uint4 v;
+                    if constexpr (kTwo) {
+                        v = make_uint4(__float_as_uint(o[e] * inv), __float_as_uint(o[e + 1] * inv), __float_as_uint(o[e + 2] * inv),
+                                       __float_as_uint(o[e + 3] * inv));
+                    } else {
+                        v = make_uint4(pack16<T>(o[e] * inv, o[e + 1] * inv), pack16<T>(o[e + 2] * inv, o[e + 3] * inv),
+                                       pack16<T>(o[e + 4] * inv, o[e + 5] * inv), pack16<T>(o[e + 6] * inv, o[e + 7] * inv));
+                    }
+                    *reinterpret_cast<uint4*>(stage + lane * (D * (int)sizeof(T)) + ((((c + e) / N) ^ lane) % kChunks) * 16) = v;
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll 4
+        for (int i0 = 0; i0 < 32; i0 += kRowsPerStore) {
+            const int i = i0 + lane / kChunks, k = lane % kChunks;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (have)
+                v = *reinterpret_cast<const uint4*>(base_ptr + t * S::kQTile + qq * (32 * D * (int)sizeof(T)) + i * (D * (int)sizeof(T)) +
+                                                    ((k ^ i) % kChunks) * 16);
+            if (row_live(i)) *reinterpret_cast<uint4*>(out + row_at(i) + k * N) = v;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+    if (s_poison) recompute_rows<T, D>(p, seq, tok0, head0);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+    });
+    return fn;
+}
+
+// A map of 16-bit values with 128-byte swizzle: boxes of 64 columns.
+mg_status map_16bit(CUtensorMap* map, mg_dtype t, const void* ptr, int rank, const uint64_t* dims, const uint64_t* strides,
+                    const uint32_t* box) {
+    auto fn = encode_fn();
+    if (!fn) return fail(MG_DRIVER_FAILED, "the driver does not provide cuTensorMapEncodeTiled");
+    cuuint64_t d[3], s[2];
+    cuuint32_t b[3], e[3] = {1, 1, 1};
+    for (int i = 0; i < rank; i++) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i > 0) s[i - 1] = strides[i - 1];
+    }
+    const CUresult r = fn(map, t == MG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank,
+                          const_cast<void*>(ptr), d, s, b, e, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(MG_DRIVER_FAILED, "encoding a TMA descriptor failed (CUresult %d)", (int)r);
+    return MG_OK;
+}
+
+template <typename T, int D>
+mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
+    using S = Shape<T, D>;
+    static_assert(S::kSmem <= 227 * 1024 - 512, "shared memory budget");
+    static bool configured[64] = {false};
+    if (!configured[d->ordinal & 63]) {
+        MG_CUDA(cudaFuncSetAttribute(attention_packed_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
+                "configuring the packed attention kernel");
+        configured[d->ordinal & 63] = true;
+    }
+    Params p;
+    p.a = a;
+    const uint32_t group = (uint32_t)(a.head_count / a.kv_head_count);
+    p.pack = 1;
+    p.pack_log2 = 0;
+    while (p.pack < 64 && group % (2 * p.pack) == 0) p.pack *= 2, p.pack_log2++;
+    p.groups = (uint32_t)a.head_count / p.pack;
+    p.tokens = 2 * kRows / p.pack;
+    p.scale2 = a.scale * 1.4426950408889634f;
+    p.error = d->flags + 2;
+    uint64_t items = 0;
+    for (const SeqRow& r : a.host->rows) items += (r.q_count + p.tokens - 1) / p.tokens;
+    if (items * p.groups > 0x7fffffffull) return fail(MG_SHAPE_UNSUPPORTED, "attention launch size overflows");
+    const uint64_t width = a.kv_head_count * D;
+    CUtensorMap maps[5];
+    const uint32_t kv_box[2] = {64, (uint32_t)S::kKeys};
+    const uint64_t kv_stride[1] = {width * 2};
+    if constexpr (S::kTerms == 2) {
+        const uint64_t keys = a.host->keys + a.max_step * a.host->rows.size();
+        uint16_t* ws = nullptr;
+        MG_TRY(scratch(d, 8, std::max<uint64_t>(keys, 1) * width * 4 * sizeof(uint16_t), (void**)&ws));
+        uint16_t* terms[4];
+        for (int i = 0; i < 4; i++) terms[i] = ws + (uint64_t)i * keys * width;
+        if (keys) {
+            const uint32_t vecs = (uint32_t)(width / 4);
+            const unsigned grid = (unsigned)std::min<uint64_t>((keys * vecs + 255) / 256, (uint64_t)d->sm_count * 16);
+            for (int i = 0; i < 2; i++) {
+                enqueue(d, split_rows_kernel, grid, 256, 0, a.table, (const float*)(i ? a.v : a.k), terms[2 * i], terms[2 * i + 1],
+                        a.host->keys, vecs);
+                MG_TRY(launched(d, "packed attention split launch"));
+            }
+        }
+        const uint64_t dims[2] = {width, std::max<uint64_t>(keys, 1)};
+        for (int i = 0; i < 4; i++) MG_TRY(map_16bit(&maps[1 + i], MG_BF16, terms[i], 2, dims, kv_stride, kv_box));
+        maps[0] = maps[1];  // queries are read by the threads that own them
+    } else {
+        const uint64_t q_dims[3] = {(uint64_t)D, a.head_count, a.queries}, q_strides[2] = {(uint64_t)D * 2, a.head_count * D * 2};
+        const uint32_t q_box[3] = {64, p.pack, (uint32_t)kRows / p.pack};
+        MG_TRY(map_16bit(&maps[0], a.dtype, a.q, 3, q_dims, q_strides, q_box));
+        const uint64_t dims[2] = {width, a.kv_rows};
+        MG_TRY(map_16bit(&maps[1], a.dtype, a.k, 2, dims, kv_stride, kv_box));
+        MG_TRY(map_16bit(&maps[3], a.dtype, a.v, 2, dims, kv_stride, kv_box));
+        maps[2] = maps[1];
+        maps[4] = maps[3];
+    }
+    enqueue(d, attention_packed_tc_kernel<T, D>, (unsigned)(items * p.groups), kThreads, S::kSmem, maps[0], maps[1], maps[2], maps[3],
+            maps[4], p);
+    return launched(d, "packed attention launch");
+}
+
+}  // namespace
+
+namespace k {
+
+// Head dimensions of whole 64-column atoms whose scores and output fit in tensor memory, on the 16-byte
+// boundaries that TMA takes; f32 also needs its split rows to be counted in 31 bits.
+bool attention_packed_tc_eligible(const PackedAttentionArgs& a) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                         reinterpret_cast<uintptr_t>(a.out);
+    return a.kv_dtype == a.dtype && (at & 15) == 0 && (a.head_dim == 64 || a.head_dim == 128) && a.value_dim == a.head_dim &&
+           a.kv_rows > 0 && (a.dtype != MG_F32 || a.host->keys + a.max_step * a.host->rows.size() < (1ull << 31));
+}
+
+mg_status attention_packed_tc(Device* d, const PackedAttentionArgs& a) {
+    return by_float(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        return a.head_dim == 64 ? launch<T, 64>(d, a) : launch<T, 128>(d, a);
+    });
+}
+
+}  // namespace k
+}  // namespace mg

@@ -126,10 +126,13 @@ struct SeqRow {
 };
 
 // The host side of a table of packed sequences (MG_SEQUENCES).  On the device the buffer holds the
-// rows and then the sequences' indices in falling order of their key counts.
+// rows, then the sequences' indices in falling order of their key counts, then for each sequence the
+// number of keys of those before it (modulo 2^32).
+constexpr uint64_t kSeqBytes = sizeof(SeqRow) + 2 * sizeof(uint32_t);  // device bytes of a sequence
 struct SequenceTable {
     std::vector<SeqRow> rows;
     uint64_t queries = 0;      // all sequences' queries
+    uint64_t keys = 0;         // all sequences' keys
     uint64_t key_end = 0;      // one past the last key row any sequence reads
     uint64_t max_queries = 0;  // of one sequence
     bool writable = true;      // no sequence has fewer keys than queries
@@ -367,11 +370,12 @@ struct AttentionArgs {
 mg_status attention(Device* d, const AttentionArgs& a);
 
 // ---- batches of packed sequences ---------------------------------------------------------
-// The table as kernels take it: `count` sequences, their order of falling key counts, and a
-// captured step's advancing key count (null: none), which every sequence's keys grow by.
+// The table as kernels take it: `count` sequences, their order of falling key counts, the keys of
+// the sequences before each, and a captured step's advancing key count (null: none), which every sequence's keys grow by.
 struct SeqTable {
     const SeqRow* rows;
     const uint32_t* order;
+    const uint32_t* key_prefix;
     uint32_t count;
     const uint64_t* step = nullptr;
 };

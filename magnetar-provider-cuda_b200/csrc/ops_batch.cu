@@ -45,6 +45,7 @@ mg_status need_table(Device* d, const mg_buffer* s, const SequenceTable** host, 
     table->rows = (const SeqRow*)b->ptr;
     table->count = (uint32_t)b->seq->rows.size();
     table->order = (const uint32_t*)(table->rows + table->count);
+    table->key_prefix = table->order + table->count;
     table->step = nullptr;
     return MG_OK;
 }
@@ -55,16 +56,15 @@ mg_status make_table(uint64_t count, const uint64_t* query_counts, const uint64_
     constexpr uint64_t kLimit = 1ull << 31;
     if (count == 0 || count >= (1u << 24)) return fail(MG_SHAPE_UNSUPPORTED, "a table cannot hold %llu sequences", (ull)count);
     t->rows.resize(count);
-    uint64_t keys = 0;
     for (uint64_t i = 0; i < count; i++) {
         const uint64_t n = query_counts[i], m = key_counts ? key_counts[i] : n;
         if (n >= kLimit || m >= kLimit) return fail(MG_SHAPE_UNSUPPORTED, "sequence %llu has 2^31 rows or more", (ull)i);
-        const uint64_t at = key_starts ? key_starts[i] : keys;
+        const uint64_t at = key_starts ? key_starts[i] : t->keys;
         if (t->queries + n >= kLimit || at >= kLimit || at + m >= kLimit)
             return fail(MG_SHAPE_UNSUPPORTED, "the rows of sequence %llu do not lie below 2^31", (ull)i);
         t->rows[i] = {(uint32_t)t->queries, (uint32_t)n, (uint32_t)at, (uint32_t)m};
         t->queries += n;
-        keys += m;
+        t->keys += m;
         t->key_end = std::max(t->key_end, at + m);
         t->max_queries = std::max(t->max_queries, n);
         if (m < n) t->writable = false;
@@ -86,11 +86,16 @@ mg_status make_table(uint64_t count, const uint64_t* query_counts, const uint64_
 mg_status upload_table(Device* d, Buffer* b) {
     const SequenceTable& t = *b->seq;
     const size_t n = t.rows.size();
-    std::vector<uint32_t> words(n * 5);
+    std::vector<uint32_t> words(n * kSeqBytes / sizeof(uint32_t));
     memcpy(words.data(), t.rows.data(), n * sizeof(SeqRow));
     uint32_t* order = words.data() + 4 * n;
     std::iota(order, order + n, 0u);
     std::stable_sort(order, order + n, [&](uint32_t x, uint32_t y) { return t.rows[x].k_count > t.rows[y].k_count; });
+    uint32_t keys = 0;
+    for (size_t i = 0; i < n; i++) {
+        order[n + i] = keys;
+        keys += t.rows[i].k_count;
+    }
     // pageable memory: the copy has read it when the call returns
     MG_CUDA(cudaMemcpyAsync(b->ptr, words.data(), words.size() * 4, cudaMemcpyHostToDevice, d->stream), "uploading a table");
     d->uploads.fetch_add(1);
@@ -266,7 +271,7 @@ mg_status mg_sequences_create(mg_device* h, uint64_t count, const uint64_t* quer
         MG_TRY(make_table(count, query_counts, key_counts, key_starts, &t));
         const uint64_t shape[2] = {count, 4};
         Buffer* b = nullptr;
-        MG_TRY(buffer_new_opaque(d, MG_SEQUENCES, 2, shape, count * (sizeof(SeqRow) + sizeof(uint32_t)), &b));
+        MG_TRY(buffer_new_opaque(d, MG_SEQUENCES, 2, shape, count * kSeqBytes, &b));
         mg_status s = MG_EXECUTION_FAILED;
         try {
             b->seq = new SequenceTable(std::move(t));

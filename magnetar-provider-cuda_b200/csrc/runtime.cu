@@ -255,7 +255,7 @@ mg_status buffer_new_opaque(Device* d, mg_dtype dtype, int rank, const uint64_t*
 
 mg_status buffer_clone_opaque(Device* d, const Buffer* src, Buffer** out) {
     const uint64_t bytes = src->dtype == MG_Q4 ? q4_bytes(src->shape[0], src->shape[1])
-                                               : src->seq->rows.size() * (sizeof(SeqRow) + sizeof(uint32_t));
+                                               : src->seq->rows.size() * kSeqBytes;
     Buffer* b = nullptr;
     MG_TRY(buffer_new_opaque(d, src->dtype, src->rank, src->shape, bytes, &b));
     if (src->seq) {

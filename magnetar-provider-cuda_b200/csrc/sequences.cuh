@@ -37,6 +37,35 @@ __device__ __forceinline__ uint32_t seq_of_query(const k::SeqTable& t, uint32_t 
     return lo;
 }
 
+// Work item `item` of a launch that gives sequence i `items_of(row i)` items, sequences with the most
+// keys first: the sequence and the item's place in it.  All lanes of a warp call it together; false
+// past the last item.
+template <class F>
+__device__ __forceinline__ bool find_item(const k::SeqTable& t, uint32_t item, F&& items_of, uint32_t& seq, uint32_t& place) {
+    const uint32_t lane = threadIdx.x % 32;
+    uint32_t before = 0;
+    for (uint32_t base = 0; base < t.count; base += 32) {
+        const uint32_t i = base + lane;
+        const uint32_t id = i < t.count ? __ldg(t.order + i) : 0;
+        const uint32_t n = i < t.count ? items_of(id) : 0;
+        uint32_t sum = n;  // items of the lanes up to this one
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= (uint32_t)o) sum += v;
+        }
+        const uint32_t owner = __ballot_sync(0xffffffffu, item < before + sum);
+        if (owner) {
+            const int l = __ffs(owner) - 1;
+            seq = __shfl_sync(0xffffffffu, id, l);
+            place = item - before - __shfl_sync(0xffffffffu, sum - n, l);
+            return true;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return false;
+}
+
 // One dtype's kernel by a generic lambda: f(T{}).
 template <class F>
 inline mg_status by_float(mg_dtype t, F&& f) {
