@@ -40,12 +40,16 @@ using namespace sm100;
 
 constexpr int kRows = 128;      // rows of a query tile (MMA M)
 constexpr int kThreads = 384;   // 12 warps
+// Registers of a thread of warps 0-3 and of warps 4-11; their sum over the block must not pass what it
+// is launched with (checked before the first launch).
+constexpr int kFewRegs = 80, kManyRegs = 200;
 
 template <typename T, int D>
 struct Shape {
     static constexpr int kTerms = sizeof(T) == 4 ? 2 : 1;
     static constexpr int kKeys = kTerms == 2 ? 64 : 128;   // keys of a tile
     static constexpr int kScores = 128 / kKeys;            // score buffers of a query tile
+    static constexpr int kParts = kKeys / 32;              // weights of a tile are handed over 32 keys at a time
     static constexpr int kQAtom = kRows * 128;             // [128 rows][64 columns], 128-byte swizzle
     static constexpr int kQTerm = (D / 64) * kQAtom;
     static constexpr int kQTile = kTerms * kQTerm;
@@ -79,6 +83,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
+}
+
+__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
 }
 
 // Two values as a packed pair of the 16-bit type, the first in the low half.
@@ -154,7 +164,7 @@ __device__ __noinline__ void recompute_rows(const Params& p, const SeqRow& s, ui
     const int lane = threadIdx.x % 32;
     const uint64_t w = p.a.kv_head_count * D;
     const PlainRows<T> kr{(const T*)p.a.k, w}, vr{(const T*)p.a.v, w};
-    for (uint32_t r = threadIdx.x / 32; r < 2 * kRows; r += kThreads / 32) {
+    for (uint32_t r = threadIdx.x / 32 - 4; r < 2 * kRows; r += 8) {  // (by warps 4-11)
         const uint32_t tok = tok0 + (r >> p.pack_log2);
         if (tok >= s.q_count) break;
         attention_row<T, PlainRows<T>, D / 32>(p.a, kr, vr, s, s.q_start + tok, head0 + (r & (p.pack - 1)), lane);
@@ -174,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr float kLazy = kFormat == 0 ? 7.0f : 8.0f;
     constexpr float kOffset = kFormat == 0 ? -8.0f : 40.0f;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ uint64_t bars[24];
+    __shared__ uint64_t bars[28];
     __shared__ uint32_t tmem_slot;
     __shared__ uint32_t s_seq, s_place, s_poison;
     const uint32_t raw = smem_u32(smem_raw);
@@ -188,15 +198,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto v_ready = [&](int s) { return b0 + 56 + 8u * (uint32_t)s; };
     auto v_empty = [&](int s) { return b0 + 72 + 8u * (uint32_t)s; };
     auto s_full = [&](int t, int b) { return b0 + 88 + 8u * (uint32_t)(2 * t + b); };
-    auto p_full = [&](int t, int b) { return b0 + 120 + 8u * (uint32_t)(2 * t + b); };
-    auto pv_done = [&](int t, int b) { return b0 + 152 + 8u * (uint32_t)(2 * t + b); };
+    auto pv_done = [&](int t, int b) { return b0 + 120 + 8u * (uint32_t)(2 * t + b); };
+    // (kScores * kParts = 4 parts of a query tile at a time)
+    auto p_full = [&](int t, int b, int part) { return b0 + 152 + 8u * (uint32_t)(4 * t + b * S::kParts + part); };
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 23; i++) {
+        for (int i = 0; i < 27; i++) {
             const uint32_t bar = b0 + 8u * (uint32_t)i;
             // P: the tile's four softmax warps; Q: all eight where they split it; V: its two warps
-            const bool is_p = bar >= p_full(0, 0) && bar <= p_full(1, 1), is_v = bar >= v_ready(0) && bar <= v_ready(1);
+            const bool is_p = bar >= p_full(0, 0, 0), is_v = bar >= v_ready(0) && bar <= v_ready(1);
             mbar_init(bar, is_p ? 4 : is_v ? 2 : bar == q_full && kTwo ? 8 : 1);
         }
         s_poison = 0;
@@ -249,6 +260,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int all_lo = window > 0 ? max(0, shift + (int)tok0 + live_tokens - window) : 0;
     const int all_hi = p.a.causal ? min(m_keys, shift + (int)tok0 + 1) : m_keys;
 
+    // The softmax threads hold a row of scores each: they take registers from the other warps.
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
     if (warp == 0) {
         // ---- TMA producer ----------------------------------------------------------------------
         if (lane == 0 && n_kv > 0) {
@@ -327,26 +341,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 bool k_ready = false;
                 for (int t = 0; t < 2 && ok; t++) {
                     if (j < n_t[t]) {
-                        ok = mbar_wait(p_full(t, j % S::kScores), (uint32_t)(j / S::kScores) & 1u);
-                        if (!ok) break;
-                        tc_fence_after();
                         // O_t += P_t(j) V(j): P from tensor memory, two values per column
                         const uint32_t tP = tmem + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
                         const uint32_t tO = tmem + S::kColO + (uint32_t)(D * t);
                         const uint64_t dv = dv0 + (uint64_t)((vs * S::kStage) >> 4);
+                        for (int part = 0; part < S::kParts; part++) {
+                            ok = mbar_wait(p_full(t, j % S::kScores, part), (uint32_t)(j / S::kScores) & 1u);
+                            if (!ok) break;
+                            tc_fence_after();
 #pragma unroll
-                        for (int kk = 0; kk < KV / 16; kk++) {
-                            const uint64_t v = dv + (uint64_t)((kk * 2048) >> 4);
-                            const uint32_t pa = tP + (uint32_t)kk * 8;
-                            const uint32_t acc = (j > 0 || kk > 0) ? 1u : 0u;
-                            if constexpr (kTwo) {
-                                mma_bf16_ts(tO, pa + KV / 2, v, idesc_o, acc);
-                                mma_bf16_ts(tO, pa, v + (uint64_t)(S::kTerm >> 4), idesc_o, 1u);
-                                mma_bf16_ts(tO, pa, v, idesc_o, 1u);
-                            } else {
-                                mma_bf16_ts(tO, pa, v, idesc_o, acc);
+                            for (int k2 = 0; k2 < 2; k2++) {
+                                const int kk = 2 * part + k2;
+                                const uint64_t v = dv + (uint64_t)((kk * 2048) >> 4);
+                                const uint32_t pa = tP + (uint32_t)kk * 8;
+                                const uint32_t acc = (j > 0 || kk > 0) ? 1u : 0u;
+                                if constexpr (kTwo) {
+                                    mma_bf16_ts(tO, pa + KV / 2, v, idesc_o, acc);
+                                    mma_bf16_ts(tO, pa, v + (uint64_t)(S::kTerm >> 4), idesc_o, 1u);
+                                    mma_bf16_ts(tO, pa, v, idesc_o, 1u);
+                                } else {
+                                    mma_bf16_ts(tO, pa, v, idesc_o, acc);
+                                }
                             }
                         }
+                        if (!ok) break;
                         tc_commit(pv_done(t, j & 1));
                     }
                     if (t == 1) tc_commit(v_empty(vs));
@@ -365,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) atomicExch(p.error, 1);
         }
         __syncwarp();
-    } else if (warp < 4) {
+    } else {
         // ---- values of tiles some row sees only in part ------------------------------------------
         const int i0 = (int)threadIdx.x - 64;
         constexpr uint32_t kExponents = kFormat == 0 ? 0x7c00u : 0x7f80u;
@@ -405,7 +423,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_arrive_warp(v_ready(s));
         }
         if (failed && lane == 0) atomicExch(p.error, 1);
+    }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
         // ---- softmax: one query row per thread ---------------------------------------------------
         const float kNegInf = __int_as_float(0xff800000);
         const int t = (warp - 4) / 4, qq = warp % 4;
@@ -495,21 +515,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 m = tmax;
                 l *= f;
             }
-            // (no key seen yet: every score is -inf, and weights 2^(-inf) are 0)
-            const float ref = m == kNegInf ? 0.0f : -(m + kOffset);
-            const uint64_t sc2 = f2(sc, sc), ref2 = f2(ref, ref);
-            float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int c = 0; c < KV; c += 2) {
-                uint64_t x = ref2;
-                f2fma(x, f2(s[c], s[c + 1]), sc2);
-                const float2 e = f2split(x);
-                s[c] = ex2(e.x);
-                s[c + 1] = ex2(e.y);
-                ps[c & 2] += s[c];
-                ps[(c & 2) + 1] += s[c + 1];
-            }
-            l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
             if (j > 0 && __any_sync(0xffffffffu, move)) {
                 // O *= f, once P V(j - 1) has completed
                 failed = !mbar_wait(pv_done(t, (j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u);
@@ -529,24 +534,41 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 tc_wait_st();
             }
-            // P over the scores just read
+            // (no key seen yet: every score is -inf, and weights 2^(-inf) are 0)
+            const float ref = m == kNegInf ? 0.0f : -(m + kOffset);
+            const uint64_t sc2 = f2(sc, sc), ref2 = f2(ref, ref);
+            uint64_t sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
 #pragma unroll
-            for (int c = 0; c < KV; c += 32) {
+            for (int part = 0; part < S::kParts; part++) {
+                // 32 weights, over the scores just read
                 uint32_t h[16];
 #pragma unroll
-                for (int e = 0; e < 16; e++) h[e] = pack16<T>(s[c + 2 * e], s[c + 2 * e + 1]);
-                tmem_st16(tS + (uint32_t)(c / 2), h);
+                for (int e = 0; e < 16; e++) {
+                    const int c = part * 32 + 2 * e;
+                    uint64_t x = ref2;
+                    f2fma(x, f2(s[c], s[c + 1]), sc2);
+                    const float2 y = f2split(x);
+                    s[c] = ex2(y.x);
+                    s[c + 1] = ex2(y.y);
+                    sum[e & 1] = f2add(sum[e & 1], f2(s[c], s[c + 1]));
+                    h[e] = pack16<T>(s[c], s[c + 1]);
+                }
+                tmem_st16(tS + (uint32_t)(part * 16), h);
                 if constexpr (kTwo) {
                     uint32_t lo[16];
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        lo[e] = pack16<T>(s[c + 2 * e] - __uint_as_float(h[e] << 16), s[c + 2 * e + 1] - __uint_as_float(h[e] & 0xffff0000u));
-                    tmem_st16(tS + (uint32_t)(KV / 2 + c / 2), lo);
+                    for (int e = 0; e < 16; e++) {
+                        const int c = part * 32 + 2 * e;
+                        lo[e] = pack16<T>(s[c] - __uint_as_float(h[e] << 16), s[c + 1] - __uint_as_float(h[e] & 0xffff0000u));
+                    }
+                    tmem_st16(tS + (uint32_t)(KV / 2 + part * 16), lo);
                 }
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive_warp(p_full(t, j % S::kScores, part));
             }
-            tc_wait_st();
-            tc_fence_before();
-            mbar_arrive_warp(p_full(t, j % S::kScores));
+            const float2 u = f2split(f2add(sum[0], sum[1]));
+            l += u.x + u.y;
         }
         // ---- the output row: O / l ---------------------------------------------------------------
         bool have = false;
@@ -605,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (s_poison) recompute_rows<T, D>(p, seq, tok0, head0);
+    if (s_poison && warp >= 4) recompute_rows<T, D>(p, seq, tok0, head0);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -648,6 +670,10 @@ mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
     if (!configured[d->ordinal & 63]) {
         MG_CUDA(cudaFuncSetAttribute(attention_packed_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
                 "configuring the packed attention kernel");
+        cudaFuncAttributes fa;
+        MG_CUDA(cudaFuncGetAttributes(&fa, attention_packed_tc_kernel<T, D>), "configuring the packed attention kernel");
+        if (fa.numRegs * kThreads < kFewRegs * 128 + kManyRegs * 256)
+            return fail(MG_EXECUTION_FAILED, "the packed attention kernel was built with %d registers, too few to share out", fa.numRegs);
         configured[d->ordinal & 63] = true;
     }
     Params p;
