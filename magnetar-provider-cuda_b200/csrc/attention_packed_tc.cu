@@ -79,9 +79,10 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// The largest of three; NaN if one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
@@ -100,12 +101,13 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
     return r;
 }
 
-// x as two bfloat16 terms; a finite value that would round to infinity is cut instead.
-__device__ __forceinline__ void split(float x, uint16_t& hi, uint16_t& lo) {
-    __nv_bfloat16 h = __float2bfloat16_rn(x);
-    if (isinf(__bfloat162float(h)) && !isinf(x)) h = __ushort_as_bfloat16((uint16_t)(__float_as_uint(x) >> 16));
-    hi = __bfloat16_as_ushort(h);
-    lo = __bfloat16_as_ushort(__float2bfloat16_rn(x - __bfloat162float(h)));
+// Two values as two bfloat16 terms each, packed; a finite value that would round to infinity is held at
+// the largest bfloat16, so that its lo term has the rest.
+__device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& lo) {
+    constexpr float kMost = 3.3895313892515355e38f;
+    const uint32_t hi = pack16<__nv_bfloat16>(fminf(fmaxf(x, -kMost), kMost), fminf(fmaxf(y, -kMost), kMost));
+    lo = pack16<__nv_bfloat16>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
+    return hi;
 }
 
 // The sequences' f32 rows, one sequence after another, as their two terms.  Streaming: 4 bytes read and
@@ -125,13 +127,11 @@ __global__ void __launch_bounds__(256) split_rows_kernel(k::SeqTable t, const fl
         }
         const uint64_t row = (uint64_t)__ldg(&t.rows[a].k_start) + (g - (__ldg(t.key_prefix + a) + (uint32_t)step * a));
         const float4 x = reinterpret_cast<const float4*>(src)[row * vecs + c];
-        uint16_t h[4], l[4];
-        split(x.x, h[0], l[0]);
-        split(x.y, h[1], l[1]);
-        split(x.z, h[2], l[2]);
-        split(x.w, h[3], l[3]);
-        reinterpret_cast<uint2*>(hi)[w] = make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
-        reinterpret_cast<uint2*>(lo)[w] = make_uint2(l[0] | (uint32_t)l[1] << 16, l[2] | (uint32_t)l[3] << 16);
+        uint2 h, l;
+        h.x = split2(x.x, x.y, l.x);
+        h.y = split2(x.z, x.w, l.y);
+        reinterpret_cast<uint2*>(hi)[w] = h;
+        reinterpret_cast<uint2*>(lo)[w] = l;
     }
 }
 
@@ -157,6 +157,46 @@ __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t next)
 constexpr uint32_t idesc(int format, int m, int n, bool b_mn) {
     return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
            ((uint32_t)(m >> 4) << 24);
+}
+
+// 1 in one lane of the warp.
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r;
+}
+
+// The MMAs and the commit, carried out by the lane whose `lead` is 1 (all lanes of the warp call them
+// with the same other arguments).
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t lead, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(lead)
+        : "memory");
 }
 
 template <typename T, int D>
@@ -201,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto pv_done = [&](int t, int b) { return b0 + 120 + 8u * (uint32_t)(2 * t + b); };
     // (kScores * kParts = 4 parts of a query tile at a time)
     auto p_full = [&](int t, int b, int part) { return b0 + 152 + 8u * (uint32_t)(4 * t + b * S::kParts + part); };
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 27; i++) {
@@ -262,168 +302,176 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // The softmax threads hold a row of scores each: they take registers from the other warps.
     if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
-    if (warp == 0) {
-        // ---- TMA producer ----------------------------------------------------------------------
-        if (lane == 0 && n_kv > 0) {
-            if constexpr (!kTwo) {
-                mbar_arrive_expect_tx(q_full, 2 * S::kQTile);
-                for (int t = 0; t < 2; t++)
-                    for (int a = 0; a < D / 64; a++)
-                        tma_load_3d(base + t * S::kQTile + a * S::kQAtom, &map_q, q_full, a * 64, (int)head0,
-                                    (int)(seq.q_start + tok0) + t * (int)p.tokens / 2);
-            }
-            auto load = [&](uint32_t slot, uint32_t bar, const CUtensorMap* hi, const CUtensorMap* lo, int j) {
-                mbar_arrive_expect_tx(bar, S::kStage);
-                for (int a = 0; a < D / 64; a++) {
-                    const int x = kvh * D + a * 64, y = key_row0 + kv0 + j * KV;
-                    tma_load_2d(slot + a * S::kAtom, hi, bar, x, y);
-                    if constexpr (kTwo) tma_load_2d(slot + S::kTerm + a * S::kAtom, lo, bar, x, y);
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewRegs));
+        if (warp == 0) {
+            // ---- TMA producer ----------------------------------------------------------------------
+            if (lane == 0 && n_kv > 0) {
+                if constexpr (!kTwo) {
+                    mbar_arrive_expect_tx(q_full, 2 * S::kQTile);
+                    for (int t = 0; t < 2; t++)
+                        for (int a = 0; a < D / 64; a++)
+                            tma_load_3d(base + t * S::kQTile + a * S::kQAtom, &map_q, q_full, a * 64, (int)head0,
+                                        (int)(seq.q_start + tok0) + t * (int)p.tokens / 2);
                 }
-            };
-            auto load_k = [&](int j) -> bool {
-                const int s = j % S::kKStages;
-                if (j >= S::kKStages && !mbar_wait(k_empty(s), (uint32_t)(j / S::kKStages - 1) & 1u)) return false;
-                load(base + S::kOffK + s * S::kStage, k_full(s), &map_k, &map_klo, j);
-                return true;
-            };
-            bool ok = load_k(0);
-            for (int j = 0; j < n_kv && ok; j++) {
-                if (j + 1 < n_kv) ok = load_k(j + 1);
+                auto load = [&](uint32_t slot, uint32_t bar, const CUtensorMap* hi, const CUtensorMap* lo, int j) {
+                    mbar_arrive_expect_tx(bar, S::kStage);
+                    for (int a = 0; a < D / 64; a++) {
+                        const int x = kvh * D + a * 64, y = key_row0 + kv0 + j * KV;
+                        tma_load_2d(slot + a * S::kAtom, hi, bar, x, y);
+                        if constexpr (kTwo) tma_load_2d(slot + S::kTerm + a * S::kAtom, lo, bar, x, y);
+                    }
+                };
+                auto load_k = [&](int j) -> bool {
+                    const int s = j % S::kKStages;
+                    if (j >= S::kKStages && !mbar_wait(k_empty(s), (uint32_t)(j / S::kKStages - 1) & 1u)) return false;
+                    load(base + S::kOffK + s * S::kStage, k_full(s), &map_k, &map_klo, j);
+                    return true;
+                };
+                bool ok = load_k(0);
+                for (int j = 0; j < n_kv && ok; j++) {
+                    if (j + 1 < n_kv) ok = load_k(j + 1);
+                    const int s = j % S::kVStages;
+                    if (ok && j >= S::kVStages) ok = mbar_wait(v_empty(s), (uint32_t)(j / S::kVStages - 1) & 1u);
+                    if (ok) load(base + S::kOffV + s * S::kStage, v_full(s), &map_v, &map_vlo, j);
+                }
+                if (!ok) atomicExch(p.error, 1);
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            // ---- MMA issuer --------------------------------------------------------------------------
+            // The whole warp walks the loop and one elected lane's instructions take effect: addresses and
+            // descriptors are then the same for all lanes and stay in uniform registers.  (Issued from a
+            // branch that one lane takes, each MMA cost some 60 cycles of moving them there.)
+            if (n_kv > 0) {
+                constexpr uint32_t idesc_s = idesc(kFormat, kRows, KV, false);
+                constexpr uint32_t idesc_o = idesc(kFormat, kRows, D, true);
+                const uint32_t lead = elected();
+                const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+                const uint32_t n0 = (uint32_t)__shfl_sync(0xffffffffu, n_t[0], 0), n1 = (uint32_t)__shfl_sync(0xffffffffu, n_t[1], 0);
+                const uint32_t n_all = max(n0, n1);
+                const uint64_t dq0 = desc_k_sw128(base), dk0 = desc_k_sw128(base + S::kOffK);
+                const uint64_t dv0 = desc_mn_sw128(base + S::kOffV, S::kAtom);
+                // S_t(j) = Q_t K(j)^T into tile t's score buffer j % kScores
+                auto issue_s = [&](uint32_t t, uint32_t j) {
+                    const uint32_t tS = tm + 128u * t + (j % S::kScores) * KV;
+                    const uint64_t dq = dq0 + (uint64_t)(t * (S::kQTile >> 4));
+                    const uint64_t dk = dk0 + (uint64_t)((j % S::kKStages) * (S::kStage >> 4));
+#pragma unroll
+                    for (int kk = 0; kk < D / 16; kk++) {
+                        const uint64_t q = dq + (uint64_t)(((kk / 4) * S::kQAtom + (kk % 4) * 32) >> 4);
+                        const uint64_t k = dk + (uint64_t)(((kk / 4) * S::kAtom + (kk % 4) * 32) >> 4);
+                        if constexpr (kTwo) {
+                            mma_ss(lead, tS, q + (uint64_t)(S::kQTerm >> 4), k, idesc_s, kk > 0 ? 1u : 0u);
+                            mma_ss(lead, tS, q, k + (uint64_t)(S::kTerm >> 4), idesc_s, 1u);
+                            mma_ss(lead, tS, q, k, idesc_s, 1u);
+                        } else {
+                            mma_ss(lead, tS, q, k, idesc_s, kk > 0 ? 1u : 0u);
+                        }
+                    }
+                    commit(lead, s_full((int)t, (int)(j % S::kScores)));
+                };
+                bool ok = mbar_wait(q_full, 0);
+                for (uint32_t j = 0; j < S::kScores && j < n_all && ok; j++) {
+                    ok = mbar_wait(k_full((int)j), 0);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (j < n0) issue_s(0, j);
+                    if (j < n1) issue_s(1, j);
+                    commit(lead, k_empty((int)j));
+                }
+                for (uint32_t j = 0; j < n_all && ok; j++) {
+                    const uint32_t vs = j % S::kVStages, jn = j + S::kScores, vp = (j / S::kVStages) & 1u;
+                    ok = mbar_wait(v_full((int)vs), vp) && mbar_wait(v_ready((int)vs), vp);
+                    if (ok && jn < n_all) ok = mbar_wait(k_full((int)(jn % S::kKStages)), (jn / S::kKStages) & 1u);
+                    if (!ok) break;
+#pragma unroll
+                    for (uint32_t t = 0; t < 2; t++) {
+                        if (j < (t ? n1 : n0)) {
+                            // O_t += P_t(j) V(j): P from tensor memory, two values per column
+                            const uint32_t tP = tm + 128u * t + (j % S::kScores) * KV;
+                            const uint32_t tO = tm + S::kColO + D * t;
+                            const uint64_t dv = dv0 + (uint64_t)(vs * (S::kStage >> 4));
+#pragma unroll
+                            for (int part = 0; part < S::kParts; part++) {
+                                ok = ok && mbar_wait(p_full((int)t, (int)(j % S::kScores), part), (j / S::kScores) & 1u);
+                                if (!ok) break;
+                                tc_fence_after();
+#pragma unroll
+                                for (int k2 = 0; k2 < 2; k2++) {
+                                    const int kk = 2 * part + k2;
+                                    const uint64_t v = dv + (uint64_t)((kk * 2048) >> 4);
+                                    const uint32_t pa = tP + (uint32_t)kk * 8;
+                                    const uint32_t acc = (j > 0 || kk > 0) ? 1u : 0u;
+                                    if constexpr (kTwo) {
+                                        mma_ts(lead, tO, pa + KV / 2, v, idesc_o, acc);
+                                        mma_ts(lead, tO, pa, v + (uint64_t)(S::kTerm >> 4), idesc_o, 1u);
+                                        mma_ts(lead, tO, pa, v, idesc_o, 1u);
+                                    } else {
+                                        mma_ts(lead, tO, pa, v, idesc_o, acc);
+                                    }
+                                }
+                            }
+                            if (!ok) break;
+                            commit(lead, pv_done((int)t, (int)(j & 1)));
+                        }
+                        if (t == 1) commit(lead, v_empty((int)vs));
+                        // With one score buffer a tile's next scores follow its own product, so that its softmax
+                        // runs beside the other tile's products.  With two they are a tile ahead, and come after
+                        // both products: V's only stage is then free for longer before it is needed again.
+                        if (S::kScores == 1 && jn < (t ? n1 : n0)) issue_s(t, jn);
+                    }
+                    if (ok && S::kScores == 2) {
+                        if (jn < n0) issue_s(0, jn);
+                        if (jn < n1) issue_s(1, jn);
+                    }
+                    if (ok && jn < n_all) commit(lead, k_empty((int)(jn % S::kKStages)));
+                }
+                if (!ok && lane == 0) atomicExch(p.error, 1);
+            }
+            __syncwarp();
+        } else {
+            // ---- values of tiles some row sees only in part ------------------------------------------
+            const int i0 = (int)threadIdx.x - 64;
+            constexpr uint32_t kExponents = kFormat == 0 ? 0x7c007c00u : 0x7f807f80u, kOne = kFormat == 0 ? 0x04000400u : 0x00800080u;
+            bool failed = false;
+            for (int j = 0; j < n_kv && !failed; j++) {
                 const int s = j % S::kVStages;
-                if (ok && j >= S::kVStages) ok = mbar_wait(v_empty(s), (uint32_t)(j / S::kVStages - 1) & 1u);
-                if (ok) load(base + S::kOffV + s * S::kStage, v_full(s), &map_v, &map_vlo, j);
-            }
-            if (!ok) atomicExch(p.error, 1);
-        }
-        __syncwarp();
-    } else if (warp == 1) {
-        // ---- MMA issuer --------------------------------------------------------------------------
-        if (lane == 0 && n_kv > 0) {
-            constexpr uint32_t idesc_s = idesc(kFormat, kRows, KV, false);
-            constexpr uint32_t idesc_o = idesc(kFormat, kRows, D, true);
-            const uint64_t dq0 = desc_k_sw128(base), dk0 = desc_k_sw128(base + S::kOffK);
-            const uint64_t dv0 = desc_mn_sw128(base + S::kOffV, S::kAtom);
-            // S_t(j) = Q_t K(j)^T into tile t's score buffer j % kScores
-            auto issue_s = [&](int t, int j) {
-                const uint32_t tS = tmem + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
-                const uint64_t dq = dq0 + (uint64_t)((t * S::kQTile) >> 4);
-                const uint64_t dk = dk0 + (uint64_t)(((j % S::kKStages) * S::kStage) >> 4);
+                failed = !mbar_wait(v_full(s), (uint32_t)(j / S::kVStages) & 1u);
+                failed = __any_sync(0xffffffffu, failed);
+                if (failed) break;
+                const int key0 = kv0 + j * KV;
+                if (key0 < all_lo || key0 + KV > all_hi) {
+                    uint8_t* stage = base_ptr + S::kOffV + s * S::kStage;
+                    uint32_t bad = 0;
+#pragma unroll 1
+                    for (int r = i0; r < KV; r += 64) {
+                        const bool seen = key0 + r < hi_cta;
+#pragma unroll 1
+                        for (int a = 0; a < S::kTerms * (D / 64); a++) {
+                            uint4* row = reinterpret_cast<uint4*>(stage + a * S::kAtom + r * 128);
+                            // (neighbouring lanes start in different banks)
+                            if (seen) {
+                                uint4 v[8];
 #pragma unroll
-                for (int kk = 0; kk < D / 16; kk++) {
-                    const uint64_t q = dq + (uint64_t)(((kk / 4) * S::kQAtom + (kk % 4) * 32) >> 4);
-                    const uint64_t k = dk + (uint64_t)(((kk / 4) * S::kAtom + (kk % 4) * 32) >> 4);
-                    if constexpr (kTwo) {
-                        mma_bf16(tS, q + (uint64_t)(S::kQTerm >> 4), k, idesc_s, kk > 0 ? 1u : 0u);
-                        mma_bf16(tS, q, k + (uint64_t)(S::kTerm >> 4), idesc_s, 1u);
-                        mma_bf16(tS, q, k, idesc_s, 1u);
-                    } else {
-                        mma_bf16(tS, q, k, idesc_s, kk > 0 ? 1u : 0u);
-                    }
-                }
-                tc_commit(s_full(t, j % S::kScores));
-            };
-            bool ok = mbar_wait(q_full, 0);
-            for (int j = 0; j < min(S::kScores, n_kv) && ok; j++) {
-                ok = mbar_wait(k_full(j), 0);
-                if (!ok) break;
-                tc_fence_after();
-                for (int t = 0; t < 2; t++)
-                    if (j < n_t[t]) issue_s(t, j);
-                tc_commit(k_empty(j));
-            }
-            for (int j = 0; j < n_kv && ok; j++) {
-                const int vs = j % S::kVStages, jn = j + S::kScores;
-                const uint32_t vp = (uint32_t)(j / S::kVStages) & 1u;
-                ok = mbar_wait(v_full(vs), vp) && mbar_wait(v_ready(vs), vp);
-                if (!ok) break;
-                tc_fence_after();
-                bool k_ready = false;
-                for (int t = 0; t < 2 && ok; t++) {
-                    if (j < n_t[t]) {
-                        // O_t += P_t(j) V(j): P from tensor memory, two values per column
-                        const uint32_t tP = tmem + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
-                        const uint32_t tO = tmem + S::kColO + (uint32_t)(D * t);
-                        const uint64_t dv = dv0 + (uint64_t)((vs * S::kStage) >> 4);
-                        for (int part = 0; part < S::kParts; part++) {
-                            ok = mbar_wait(p_full(t, j % S::kScores, part), (uint32_t)(j / S::kScores) & 1u);
-                            if (!ok) break;
-                            tc_fence_after();
+                                for (int c = 0; c < 8; c++) v[c] = row[(c + lane) & 7];
+                                // an exponent of all ones, and only that, carries into the sign's place
 #pragma unroll
-                            for (int k2 = 0; k2 < 2; k2++) {
-                                const int kk = 2 * part + k2;
-                                const uint64_t v = dv + (uint64_t)((kk * 2048) >> 4);
-                                const uint32_t pa = tP + (uint32_t)kk * 8;
-                                const uint32_t acc = (j > 0 || kk > 0) ? 1u : 0u;
-                                if constexpr (kTwo) {
-                                    mma_bf16_ts(tO, pa + KV / 2, v, idesc_o, acc);
-                                    mma_bf16_ts(tO, pa, v + (uint64_t)(S::kTerm >> 4), idesc_o, 1u);
-                                    mma_bf16_ts(tO, pa, v, idesc_o, 1u);
-                                } else {
-                                    mma_bf16_ts(tO, pa, v, idesc_o, acc);
-                                }
-                            }
-                        }
-                        if (!ok) break;
-                        tc_commit(pv_done(t, j & 1));
-                    }
-                    if (t == 1) tc_commit(v_empty(vs));
-                    if (jn < n_t[t]) {
-                        if (!k_ready) {
-                            ok = mbar_wait(k_full(jn % S::kKStages), (uint32_t)(jn / S::kKStages) & 1u);
-                            if (!ok) break;
-                            tc_fence_after();
-                            k_ready = true;
-                        }
-                        issue_s(t, jn);
-                    }
-                }
-                if (ok && jn < n_kv) tc_commit(k_empty(jn % S::kKStages));
-            }
-            if (!ok) atomicExch(p.error, 1);
-        }
-        __syncwarp();
-    } else {
-        // ---- values of tiles some row sees only in part ------------------------------------------
-        const int i0 = (int)threadIdx.x - 64;
-        constexpr uint32_t kExponents = kFormat == 0 ? 0x7c00u : 0x7f80u;
-        bool failed = false;
-        for (int j = 0; j < n_kv && !failed; j++) {
-            const int s = j % S::kVStages;
-            failed = !mbar_wait(v_full(s), (uint32_t)(j / S::kVStages) & 1u);
-            failed = __any_sync(0xffffffffu, failed);
-            if (failed) break;
-            const int key0 = kv0 + j * KV;
-            if (key0 < all_lo || key0 + KV > all_hi) {
-                uint8_t* stage = base_ptr + S::kOffV + s * S::kStage;
-                bool bad = false;
-                for (int r = i0; r < KV; r += 64) {
-                    const bool seen = key0 + r < hi_cta;
-                    for (int a = 0; a < S::kTerms * (D / 64); a++) {
-                        uint4* row = reinterpret_cast<uint4*>(stage + a * S::kAtom + r * 128);
-#pragma unroll
-                        for (int c = 0; c < 8; c++) {
-                            uint4& v = row[(c + lane) & 7];  // (neighbouring lanes in different banks)
-                            if (!seen) {
-                                v = make_uint4(0u, 0u, 0u, 0u);
+                                for (int c = 0; c < 8; c++)
+                                    bad |= ((v[c].x & kExponents) + kOne) | ((v[c].y & kExponents) + kOne) | ((v[c].z & kExponents) + kOne) |
+                                           ((v[c].w & kExponents) + kOne);
                             } else {
-                                const uint4 x = v;
 #pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    const uint32_t u = e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w;
-                                    bad = bad || (u & kExponents) == kExponents || ((u >> 16) & kExponents) == kExponents;
-                                }
+                                for (int c = 0; c < 8; c++) row[(c + lane) & 7] = make_uint4(0u, 0u, 0u, 0u);
                             }
                         }
                     }
+                    if (bad & 0x80008000u) s_poison = 1;
+                    fence_proxy_async();  // the zeros are read by tcgen05.mma
                 }
-                if (bad) s_poison = 1;
-                fence_proxy_async();  // the zeros are read by tcgen05.mma
+                mbar_arrive_warp(v_ready(s));
             }
-            mbar_arrive_warp(v_ready(s));
+            if (failed && lane == 0) atomicExch(p.error, 1);
         }
-        if (failed && lane == 0) atomicExch(p.error, 1);
-    }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kManyRegs));
         // ---- softmax: one query row per thread ---------------------------------------------------
@@ -433,38 +481,43 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int tile_tok0 = (int)tok0 + t * (int)p.tokens / 2;
         const int tok = tile_tok0 + (r >> p.pack_log2);
         const bool live = tok < (int)seq.q_count;
-        // element offset of row i of this warp in q and out
+        // element offset of row i of this warp in q and out; of the sequence's last token past its end
         auto row_at = [&](int i) {
             const int rr = qq * 32 + i;
-            const uint64_t token = (uint64_t)seq.q_start + (uint64_t)(tile_tok0 + (rr >> p.pack_log2));
+            const uint64_t token = (uint64_t)seq.q_start + (uint64_t)min(tile_tok0 + (rr >> p.pack_log2), (int)seq.q_count - 1);
             return (token * p.a.head_count + head0 + (uint32_t)(rr & (int)(p.pack - 1))) * D;
         };
         auto row_live = [&](int i) { return tile_tok0 + ((qq * 32 + i) >> p.pack_log2) < (int)seq.q_count; };
         if constexpr (kTwo) {
             if (n_kv > 0) {
                 // This warp's 32 query rows as two terms in the MMA's K-major layout: 16-byte chunk c of a row
-                // at position c ^ (row % 8); zeros for rows past the sequence.  One row per load, each
-                // lane D / 32 columns, all rows in flight before the first is split.
+                // at position c ^ (row % 8).  Rows past the sequence repeat its last token (their outputs go
+                // nowhere), so that no load hangs on a condition: a conditional load is waited for before
+                // the next one starts.  One row per load, each lane D / 32 columns, sixteen rows in flight.
                 constexpr int V = D / 32;
                 using Vec = typename std::conditional<V == 4, float4, float2>::type;
                 const float* q = (const float*)p.a.q;
-                Vec xv[32];
-#pragma unroll
-                for (int i = 0; i < 32; i++) xv[i] = row_live(i) ? __ldg(reinterpret_cast<const Vec*>(q + row_at(i) + lane * V)) : Vec{};
                 uint8_t* qt = base_ptr + t * S::kQTile;
                 const int e0 = lane * V, a = e0 / 64, c = (e0 % 64) / 8, byte = (e0 % 8) * 2;
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32; i0 += 16) {
+                    Vec xv[16];
 #pragma unroll
-                for (int i = 0; i < 32; i++) {
-                    const int rr = qq * 32 + i;
-                    const int off = a * S::kQAtom + rr * 128 + ((c ^ (rr & 7)) * 16 + byte);
-                    const float* xs = reinterpret_cast<const float*>(&xv[i]);
-                    uint16_t h[V], l[V];
+                    for (int i = 0; i < 16; i++) {
+                        xv[i] = __ldg(reinterpret_cast<const Vec*>(q + row_at(i0 + i) + lane * V));
+                    }
 #pragma unroll
-                    for (int e = 0; e < V; e++) split(xs[e], h[e], l[e]);
+                    for (int i = 0; i < 16; i++) {
+                        const int rr = qq * 32 + i0 + i;
+                        const int off = a * S::kQAtom + rr * 128 + ((c ^ (rr & 7)) * 16 + byte);
+                        const float* xs = reinterpret_cast<const float*>(&xv[i]);
 #pragma unroll
-                    for (int e = 0; e < V; e += 2) {
-                        *reinterpret_cast<uint32_t*>(qt + off + 2 * e) = h[e] | (uint32_t)h[e + 1] << 16;
-                        *reinterpret_cast<uint32_t*>(qt + S::kQTerm + off + 2 * e) = l[e] | (uint32_t)l[e + 1] << 16;
+                        for (int e = 0; e < V; e += 2) {
+                            uint32_t lo;
+                            const uint32_t hi = split2(xs[e], xs[e + 1], lo);
+                            *reinterpret_cast<uint32_t*>(qt + off + 2 * e) = hi;
+                            *reinterpret_cast<uint32_t*>(qt + S::kQTerm + off + 2 * e) = lo;
+                        }
                     }
                 }
                 fence_proxy_async();  // the generic-proxy writes are read by tcgen05.mma
@@ -488,11 +541,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             const uint32_t tS = lane_base + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
             float s[KV];
+            const int key0 = kv0 + j * KV;
+            const bool part_seen = key0 < row_lo || key0 + KV > row_hi;
 #pragma unroll
             for (int c = 0; c < KV; c += 32) tmem_ld32(tS + (uint32_t)c, s + c);
             tc_wait_ld();
-            const int key0 = kv0 + j * KV;
-            if (key0 < row_lo || key0 + KV > row_hi) {
+            if (part_seen) {
                 const int lo = row_lo - key0, hi = row_hi - key0;
 #pragma unroll
                 for (int c = 0; c < KV; c++) s[c] = c >= lo && c < hi ? s[c] : kNegInf;
@@ -500,19 +554,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             // the row's maximum of the raw scores (sc > 0 keeps their order), in log2 units
             float mx[4];
 #pragma unroll
-            for (int g = 0; g < 4; g++) mx[g] = fmaxf(s[g], s[g + 4]);
+            for (int g = 0; g < 4; g++) mx[g] = max3(s[g], s[g + 4], s[g + 8]);
 #pragma unroll
-            for (int c = 8; c < KV; c += 8)
+            for (int c = 12; c + 4 < KV; c += 8)
 #pragma unroll
                 for (int g = 0; g < 4; g++) mx[g] = max3(mx[g], s[c + g], s[c + 4 + g]);
-            const float tmax = fmaxf(max3(mx[0], mx[1], mx[2]), mx[3]) * sc;
-            // the reference moves only when this tile's maximum passes it by more than kLazy
-            bool move = tmax != kNegInf && (m == kNegInf || tmax > m + kLazy);
+#pragma unroll
+            for (int g = 0; g < 4; g++) mx[g] = max3(mx[g], s[KV - 4 + g], s[KV - 4 + g]);
+            const float tmax = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sc;
+            // the reference moves only when this tile's maximum passes it by more than kLazy; scores that are
+            // NaN or +inf make it NaN, and with it all of the row
+            bool move = tmax != kNegInf && !(tmax <= m + kLazy);
             float f = 1.0f;
             if (move) {
                 f = m == kNegInf ? 0.0f : ex2(m - tmax);
                 move = m != kNegInf;  // an O that holds only zero weights needs no rescale
-                m = tmax;
+                m = fmaf(tmax, 0.0f, tmax);
                 l *= f;
             }
             if (j > 0 && __any_sync(0xffffffffu, move)) {
@@ -538,6 +595,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float ref = m == kNegInf ? 0.0f : -(m + kOffset);
             const uint64_t sc2 = f2(sc, sc), ref2 = f2(ref, ref);
             uint64_t sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+            auto hand_over = [&](int part) {
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive_warp(p_full(t, j % S::kScores, part));
+            };
 #pragma unroll
             for (int part = 0; part < S::kParts; part++) {
                 // 32 weights, over the scores just read
@@ -553,6 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     sum[e & 1] = f2add(sum[e & 1], f2(s[c], s[c + 1]));
                     h[e] = pack16<T>(s[c], s[c + 1]);
                 }
+                if (part > 0) hand_over(part - 1);  // (the stores before it have had this part's time)
                 tmem_st16(tS + (uint32_t)(part * 16), h);
                 if constexpr (kTwo) {
                     uint32_t lo[16];
@@ -563,10 +626,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     tmem_st16(tS + (uint32_t)(KV / 2 + part * 16), lo);
                 }
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive_warp(p_full(t, j % S::kScores, part));
             }
+            hand_over(S::kParts - 1);
             const float2 u = f2split(f2add(sum[0], sum[1]));
             l += u.x + u.y;
         }
@@ -587,10 +648,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             // reads once the last P V has completed -- with chunk k of row i at position k ^ i; then the
             // warp stores whole rows, 16 bytes per lane.
             tc_fence_after();
-            const float inv = l > 0.0f ? 1.0f / l : l != l ? l : 0.0f;
+            const float inv = m == kNegInf ? 0.0f : 1.0f / l;
             uint8_t* stage = base_ptr + t * S::kQTile + qq * (32 * D * (int)sizeof(T));
             fence_proxy_async();  // after the MMAs' reads of this area, before generic writes
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 float o[32];
                 tmem_ld32(tO + (uint32_t)c, o);
@@ -610,14 +671,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         }
-#pragma unroll 4
-        for (int i0 = 0; i0 < 32; i0 += kRowsPerStore) {
-            const int i = i0 + lane / kChunks, k = lane % kChunks;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (have)
-                v = *reinterpret_cast<const uint4*>(base_ptr + t * S::kQTile + qq * (32 * D * (int)sizeof(T)) + i * (D * (int)sizeof(T)) +
-                                                    ((k ^ i) % kChunks) * 16);
-            if (row_live(i)) *reinterpret_cast<uint4*>(out + row_at(i) + k * N) = v;
+        const uint8_t* staged = base_ptr + t * S::kQTile + qq * (32 * D * (int)sizeof(T));
+        const int chunk = lane % kChunks;
+#pragma unroll 1
+        for (int i0 = lane / kChunks; i0 < 32; i0 += 4 * kRowsPerStore) {
+            uint4 v[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int i = i0 + u * kRowsPerStore;
+                v[u] = *reinterpret_cast<const uint4*>(staged + i * (D * (int)sizeof(T)) + ((chunk ^ i) % kChunks) * 16);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int i = i0 + u * kRowsPerStore;
+                if (row_live(i)) *reinterpret_cast<uint4*>(out + row_at(i) + chunk * N) = have ? v[u] : make_uint4(0u, 0u, 0u, 0u);
+            }
         }
     }
 
