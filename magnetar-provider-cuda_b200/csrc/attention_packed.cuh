@@ -28,8 +28,7 @@ struct Q4Rows {
         const uint8_t* rec = base + (row / kQ4Tile * columns + col / kQ4Block) * kQ4Record;
         const uint32_t r = (uint32_t)(row % kQ4Tile), c = col % kQ4Block;
         const int q = (int)((rec[r * 32 + c / 2] >> (4 * (c & 1))) & 15) - 8;
-        const uint32_t slot = (r & ~15u) | ((r & 3u) << 2) | ((r >> 2) & 3u);
-        return (float)q * __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(rec + kQ4Quants)[slot]);
+        return (float)q * __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(rec + kQ4Quants)[q4_scale_slot(r)]);
     }
 };
 

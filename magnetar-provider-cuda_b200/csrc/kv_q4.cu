@@ -15,10 +15,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Where a record's scale of row r (of 64) lies: rows t, t + 4, t + 8, t + 12 of each 16 are
-// neighbours, as the attention kernel's lanes take them.
-__device__ __forceinline__ uint32_t scale_slot(uint32_t r) { return (r & ~15u) | ((r & 3u) << 2) | ((r >> 2) & 3u); }
-
 __device__ __forceinline__ uint8_t* record(void* store, uint64_t row, uint64_t columns, uint64_t column) {
     return (uint8_t*)store + (row / kQ4Tile * columns + column) * kQ4Record;
 }
@@ -90,7 +86,7 @@ __global__ void __launch_bounds__(kThreads) q4_write_kernel(const k::KvPackedArg
         uint8_t* rec = record(a.store, row, columns, c);
         const uint32_t r = (uint32_t)(row % kQ4Tile);
         reinterpret_cast<uint32_t*>(rec)[r * 8 + part] = word;
-        if (part == 0) reinterpret_cast<__nv_bfloat16*>(rec + kQ4Quants)[scale_slot(r)] = scale;
+        if (part == 0) reinterpret_cast<__nv_bfloat16*>(rec + kQ4Quants)[q4_scale_slot(r)] = scale;
     }
 }
 
@@ -107,7 +103,7 @@ __global__ void __launch_bounds__(kThreads) q4_read_kernel(const k::KvPackedArgs
         const uint8_t* rec = record(a.store, row, columns, c);
         const uint32_t r = (uint32_t)(row % kQ4Tile);
         const uint32_t word = reinterpret_cast<const uint32_t*>(rec)[r * 8 + part];
-        const float d = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(rec + kQ4Quants)[scale_slot(r)]);
+        const float d = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(rec + kQ4Quants)[q4_scale_slot(r)]);
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = (float)((int)((word >> (4 * e)) & 15u) - 8) * d;

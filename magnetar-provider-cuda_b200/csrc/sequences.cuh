@@ -66,6 +66,12 @@ __device__ __forceinline__ bool find_item(const k::SeqTable& t, uint32_t item, F
     return false;
 }
 
+// Where a 4-bit store's record keeps the scale of its row r (of 64): of each 16, rows t + 4 e and
+// t + 4 e + 8 (e = 0, 1) are neighbours, as the attention kernel's lanes take them.
+__device__ __forceinline__ uint32_t q4_scale_slot(uint32_t r) {
+    return (r & ~15u) | ((r & 3u) << 2) | ((r >> 1) & 2u) | ((r >> 3) & 1u);
+}
+
 // One dtype's kernel by a generic lambda: f(T{}).
 template <class F>
 inline mg_status by_float(mg_dtype t, F&& f) {
