@@ -262,11 +262,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         // grid order, so light ones fill the last wave.  (The table was written by copies, which a
         // launch never overtakes.)
         uint32_t seq, place;
-        auto tiles = [&](uint32_t i) { return (__ldg(&p.a.table.rows[i].q_count) + p.tokens - 1) / p.tokens; };
+        auto tiles = [&](uint32_t n) { return (n + p.tokens - 1) / p.tokens; };
         const bool found = find_item(p.a.table, blockIdx.x / p.groups, tiles, seq, place);
         if (lane == 0) {
             s_seq = found ? seq : 0xffffffffu;
-            s_place = found ? tiles(seq) - 1 - place : 0;
+            s_place = found ? tiles(__ldg(&p.a.table.ordered[seq].q_count)) - 1 - place : 0;
         }
     }
     pdl_enter();  // after the TMEM allocation, as every tensor-memory kernel here does
@@ -275,14 +275,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
     const bool any = s_seq != 0xffffffffu;
-    const SeqRow seq = any ? seq_load(p.a.table, s_seq) : SeqRow{0, 0, 0, 0};
+    const SeqRow seq = any ? seq_load(p.a.table, p.a.table.ordered, s_seq) : SeqRow{0, 0, 0, 0};
     const uint32_t tok0 = s_place * p.tokens, head0 = (blockIdx.x % p.groups) * p.pack;
     const int kvh = (int)(head0 / (uint32_t)(p.a.head_count / p.a.kv_head_count));
     const int m_keys = (int)seq.k_count, shift = m_keys - (int)seq.q_count;  // token i stands at shift + i
     const int window = p.a.window >= 0 && p.a.window < 0x7fffffff ? (int)p.a.window : -1;
     // first row of K and V: f32 terms lie in the workspace, packed
-    const int key_row0 = kTwo ? (any ? (int)(__ldg(p.a.table.key_prefix + s_seq) + (p.a.table.step ? (uint32_t)*p.a.table.step * s_seq : 0u)) : 0)
-                              : (int)seq.k_start;
+    int key_row0 = (int)seq.k_start;
+    if (kTwo && any) {
+        const uint32_t id = __ldg(p.a.table.order + s_seq);
+        key_row0 = (int)(__ldg(p.a.table.key_prefix + id) + (p.a.table.step ? (uint32_t)*p.a.table.step * id : 0u));
+    }
     // Keys [kv0, ...) the CTA reads, and the tiles of them each query tile reads.
     const int live_tokens = min((int)p.tokens, (int)seq.q_count - (int)tok0);
     const int kv0 = window > 0 ? max(0, shift + (int)tok0 - window + 1) : 0;

@@ -37,10 +37,7 @@ using namespace sm100;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 2;  // tiles of K and V a warp has in flight or in use
-#ifndef PSM
-#define PSM 3
-#endif
-constexpr int kPerSm = PSM;   // CTAs of an SM: as many as shared memory holds
+constexpr int kPerSm = 3;   // CTAs of an SM: as many as shared memory holds
 
 template <int D>
 struct Q4Shape {
@@ -151,7 +148,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
             for (int s = 0; s < kStages; s++) mbar_init(smem_u32(&bars[w][s]), 1);
         fence_barrier_init();
     }
-    pdl_enter();
+    if (tab.step) pdl_enter();  // (the table itself was written by copies, which a launch never overtakes)
     // A sequence's tiles (one at least, for a row block without keys), and its row blocks.
     auto tiles_of = [&](const SeqRow& q) { return max(1u, (uint32_t)(((uint64_t)q.k_start + q.k_count + 63) / 64 - q.k_start / 64)); };
     auto blocks_of = [&](const SeqRow& q) { return (q.q_count * p.group + R - 1) / R; };
@@ -174,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
             const uint32_t i = base + lane;
             uint64_t sum = 0;
             if (i < tab.count) {
-                const SeqRow q = seq_load(tab, __ldg(tab.order + i));
+                const SeqRow q = seq_load(tab, tab.ordered, i);
                 sum = (uint64_t)blocks_of(q) * tiles_of(q);
             }
 #pragma unroll
@@ -197,6 +194,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
             s_begin = units;
         }
     }
+    if (!tab.step) pdl_enter();
     __syncthreads();
     const uint64_t units = s_begin;
     uint64_t pos = units * blockIdx.x / gridDim.x;
@@ -212,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
 
     // ---- row blocks, or the shares of them, one after another ---------------------------------------
     while (pos < end && order < tab.count) {
-        const SeqRow seq = seq_load(tab, __ldg(tab.order + order));
+        const SeqRow seq = seq_load(tab, tab.ordered, order);
         const uint32_t all_tiles = tiles_of(seq);
         const uint64_t seq_units = (uint64_t)blocks_of(seq) * all_tiles;
         if (at >= seq_units) {  // (an empty sequence, or the last one done)
@@ -619,27 +617,38 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
                 const bool head = units * cta0 / gridDim.x == block_begin;  // the first share begins its CTA's
                 const float* parts = p.partial + (cta0 * p.a.kv_head_count + kvh) * 2 * kPart;
                 auto share = [&](uint32_t i) { return parts + i * next + (i == 0 && !head ? kPart : 0); };
-                for (int e = threadIdx.x; e < R * (D / 2); e += kThreads) {
-                    const int r = e / (D / 2), c = 2 * (e % (D / 2));
+                // Four columns of a row per thread, the shares taken in order, eight loads ahead; a running maximum
+                // as in the main loop.
+                for (int e = threadIdx.x; e < R * (D / 4); e += kThreads) {
+                    const int r = e / (D / 4), c = 4 * (e % (D / 4));
                     if (row0 + r >= rows) break;
-                    float mm = kNegInf;
-                    for (uint32_t i = 0; i < shares; i++) {
-                        const float mw = __ldcg(share(i) + r * (D + 2) + D);
-                        mm = max3(mm, mw, mw);
-                    }
-                    float ll = 0.0f, a0 = 0.0f, a1 = 0.0f;
-                    for (uint32_t i = 0; i < shares; i++) {
-                        const float* q = share(i) + r * (D + 2);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + D)), v = __ldcg(reinterpret_cast<const float2*>(q + c));
-                        const float f = ml.x == kNegInf ? 0.0f : ex2(ml.x - mm);
-                        ll = fmaf(f, ml.y, ll);
-                        a0 = fmaf(f, v.x, a0);
-                        a1 = fmaf(f, v.y, a1);
+                    float mm = kNegInf, ll = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (uint32_t i0 = 0; i0 < shares; i0 += 8) {
+                        float2 ml[8], v0[8], v1[8];
+#pragma unroll
+                        for (uint32_t u = 0; u < 8; u++) {
+                            const float* q = share(min(i0 + u, shares - 1)) + r * (D + 2);
+                            ml[u] = __ldcg(reinterpret_cast<const float2*>(q + D));
+                            v0[u] = __ldcg(reinterpret_cast<const float2*>(q + c));
+                            v1[u] = __ldcg(reinterpret_cast<const float2*>(q + c + 2));
+                        }
+#pragma unroll
+                        for (uint32_t u = 0; u < 8; u++) {
+                            if (i0 + u >= shares || ml[u].x == kNegInf) continue;
+                            const float m_new = max3(mm, ml[u].x, ml[u].x);
+                            const float f = mm == kNegInf ? 0.0f : ex2(mm - m_new), w = ex2(ml[u].x - m_new);
+                            mm = m_new;
+                            ll = fmaf(w, ml[u].y, ll * f);
+                            y[0] = fmaf(w, v0[u].x, y[0] * f);
+                            y[1] = fmaf(w, v0[u].y, y[1] * f);
+                            y[2] = fmaf(w, v1[u].x, y[2] * f);
+                            y[3] = fmaf(w, v1[u].y, y[3] * f);
+                        }
                     }
                     const float inv = mm == kNegInf ? 0.0f : 1.0f / ll;
                     T* dst = row_out(r) + c;
-                    dst[0] = from_f32<T>(a0 * inv);
-                    dst[1] = from_f32<T>(a1 * inv);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) dst[i] = from_f32<T>(y[i] * inv);
                 }
             }
         }

@@ -126,9 +126,9 @@ struct SeqRow {
 };
 
 // The host side of a table of packed sequences (MG_SEQUENCES).  On the device the buffer holds the
-// rows, then the sequences' indices in falling order of their key counts, then for each sequence the
-// number of keys of those before it (modulo 2^32).
-constexpr uint64_t kSeqBytes = sizeof(SeqRow) + 2 * sizeof(uint32_t);  // device bytes of a sequence
+// rows, then the same rows in falling order of their key counts, then the sequences' indices in that
+// order, then for each sequence the number of keys of those before it (modulo 2^32).
+constexpr uint64_t kSeqBytes = 2 * sizeof(SeqRow) + 2 * sizeof(uint32_t);  // device bytes of a sequence
 struct SequenceTable {
     std::vector<SeqRow> rows;
     uint64_t queries = 0;      // all sequences' queries
@@ -370,10 +370,11 @@ struct AttentionArgs {
 mg_status attention(Device* d, const AttentionArgs& a);
 
 // ---- batches of packed sequences ---------------------------------------------------------
-// The table as kernels take it: `count` sequences, their order of falling key counts, the keys of
-// the sequences before each, and a captured step's advancing key count (null: none), which every sequence's keys grow by.
+// The table as kernels take it: `count` sequences, the same in falling order of their key counts with
+// their indices, the keys of the sequences before each, and a captured step's advancing key count (null: none), which every sequence's keys grow by.
 struct SeqTable {
     const SeqRow* rows;
+    const SeqRow* ordered;
     const uint32_t* order;
     const uint32_t* key_prefix;
     uint32_t count;

@@ -44,7 +44,8 @@ mg_status need_table(Device* d, const mg_buffer* s, const SequenceTable** host, 
     *host = b->seq;
     table->rows = (const SeqRow*)b->ptr;
     table->count = (uint32_t)b->seq->rows.size();
-    table->order = (const uint32_t*)(table->rows + table->count);
+    table->ordered = table->rows + table->count;
+    table->order = (const uint32_t*)(table->ordered + table->count);
     table->key_prefix = table->order + table->count;
     table->step = nullptr;
     return MG_OK;
@@ -88,11 +89,12 @@ mg_status upload_table(Device* d, Buffer* b) {
     const size_t n = t.rows.size();
     std::vector<uint32_t> words(n * kSeqBytes / sizeof(uint32_t));
     memcpy(words.data(), t.rows.data(), n * sizeof(SeqRow));
-    uint32_t* order = words.data() + 4 * n;
+    uint32_t* order = words.data() + 8 * n;
     std::iota(order, order + n, 0u);
     std::stable_sort(order, order + n, [&](uint32_t x, uint32_t y) { return t.rows[x].k_count > t.rows[y].k_count; });
     uint32_t keys = 0;
     for (size_t i = 0; i < n; i++) {
+        memcpy(words.data() + 4 * (n + i), &t.rows[order[i]], sizeof(SeqRow));
         order[n + i] = keys;
         keys += t.rows[i].k_count;
     }

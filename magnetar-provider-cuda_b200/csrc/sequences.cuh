@@ -20,10 +20,12 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-__device__ __forceinline__ SeqRow seq_load(const k::SeqTable& t, uint32_t i) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(t.rows) + i);
+// A row of `rows` (of the table's rows or ordered rows), with a captured step's advance.
+__device__ __forceinline__ SeqRow seq_load(const k::SeqTable& t, const SeqRow* rows, uint32_t i) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(rows) + i);
     return SeqRow{v.x, v.y, v.z, v.w + (t.step ? (uint32_t)*t.step : 0u)};
 }
+__device__ __forceinline__ SeqRow seq_load(const k::SeqTable& t, uint32_t i) { return seq_load(t, t.rows, i); }
 
 // The sequence that owns packed query row `row` (below the table's queries): the last one that
 // starts at or before it.  Empty sequences share their start with the next one, which is later.
@@ -37,17 +39,16 @@ __device__ __forceinline__ uint32_t seq_of_query(const k::SeqTable& t, uint32_t 
     return lo;
 }
 
-// Work item `item` of a launch that gives sequence i `items_of(row i)` items, sequences with the most
-// keys first: the sequence and the item's place in it.  All lanes of a warp call it together; false
-// past the last item.
+// Work item `item` of a launch that gives a sequence of n queries `items_of(n)` items, sequences with the
+// most keys first: the sequence's place in that order and the item's place in the sequence.  All lanes of
+// a warp call it together; false past the last item.
 template <class F>
 __device__ __forceinline__ bool find_item(const k::SeqTable& t, uint32_t item, F&& items_of, uint32_t& seq, uint32_t& place) {
     const uint32_t lane = threadIdx.x % 32;
     uint32_t before = 0;
     for (uint32_t base = 0; base < t.count; base += 32) {
         const uint32_t i = base + lane;
-        const uint32_t id = i < t.count ? __ldg(t.order + i) : 0;
-        const uint32_t n = i < t.count ? items_of(id) : 0;
+        const uint32_t n = i < t.count ? items_of(__ldg(&t.ordered[i].q_count)) : 0;
         uint32_t sum = n;  // items of the lanes up to this one
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -57,7 +58,7 @@ __device__ __forceinline__ bool find_item(const k::SeqTable& t, uint32_t item, F
         const uint32_t owner = __ballot_sync(0xffffffffu, item < before + sum);
         if (owner) {
             const int l = __ffs(owner) - 1;
-            seq = __shfl_sync(0xffffffffu, id, l);
+            seq = base + l;
             place = item - before - __shfl_sync(0xffffffffu, sum - n, l);
             return true;
         }
