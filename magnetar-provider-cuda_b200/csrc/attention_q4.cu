@@ -20,7 +20,8 @@
 // is one (query, head) of a kv head.
 //
 // The tiles (64 keys on the store's own boundaries) of all sequences and row blocks form one line per kv
-// head, cut into equal shares, one per CTA: however ragged the batch, all CTAs have as much to do.  In
+// head, each row block with a length for its own cost in front, and the line is cut into equal shares,
+// one per CTA: however ragged the batch, all CTAs have as much to do.  In
 // a share a warp takes every fourth tile on its own, with its own maximum, sum and output.  The four warps'
 // results are merged in shared memory, those of a row block that was cut by the CTA that finishes last.
 #include <algorithm>
@@ -37,6 +38,7 @@ using namespace sm100;
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 2;  // tiles of K and V a warp has in flight or in use
+constexpr int kBlockCost = 12;  // a row block's queries and merge cost as much as so many tiles
 constexpr int kPerSm = 3;   // CTAs of an SM: as many as shared memory holds
 
 template <int D>
@@ -52,7 +54,7 @@ struct Q4Shape {
 struct Q4Params {
     k::PackedAttentionArgs a;
     uint32_t group;        // heads per kv head
-    uint64_t units;        // tiles of all row blocks (without a captured step's advance)
+    uint64_t units;        // of all row blocks (without a captured step's advance)
     float scale2;          // scores to log2 units
     float* partial;        // two per CTA: R x (D + 2)
     unsigned* counters;    // per CTA, for the row block that runs on past its share
@@ -134,8 +136,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
     constexpr float kLazy = 8.0f, kOffset = 40.0f;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[kWarps][kStages];
-    __shared__ uint32_t s_order, s_at;
-    __shared__ uint64_t s_begin;
+    __shared__ uint32_t s_order;
+    __shared__ uint64_t s_at, s_units;
     __shared__ uint32_t s_last;
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x / 32, 0), lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const uint32_t kvh = blockIdx.y;
@@ -149,8 +151,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
         fence_barrier_init();
     }
     if (tab.step) pdl_enter();  // (the table itself was written by copies, which a launch never overtakes)
-    // A sequence's tiles (one at least, for a row block without keys), and its row blocks.
-    auto tiles_of = [&](const SeqRow& q) { return max(1u, (uint32_t)(((uint64_t)q.k_start + q.k_count + 63) / 64 - q.k_start / 64)); };
+    // A sequence's units (its tiles, and what a row block costs beside them), and its row blocks.
+    auto units_of = [&](const SeqRow& q) { return kBlockCost + (uint32_t)(((uint64_t)q.k_start + q.k_count + 63) / 64 - q.k_start / 64); };
     auto blocks_of = [&](const SeqRow& q) { return (q.q_count * p.group + R - 1) / R; };
     if (warp == 0) {
         // The line's length, and this CTA's share of it: from unit `begin` on; then the sequence it lies in.
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
             units = 0;
             for (uint32_t i = lane; i < tab.count; i += 32) {
                 const SeqRow q = seq_load(tab, i);
-                units += (uint64_t)blocks_of(q) * tiles_of(q);
+                units += (uint64_t)blocks_of(q) * units_of(q);
             }
 #pragma unroll
             for (int w = 16; w > 0; w >>= 1) units += __shfl_xor_sync(0xffffffffu, units, w);
@@ -172,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
             uint64_t sum = 0;
             if (i < tab.count) {
                 const SeqRow q = seq_load(tab, tab.ordered, i);
-                sum = (uint64_t)blocks_of(q) * tiles_of(q);
+                sum = (uint64_t)blocks_of(q) * units_of(q);
             }
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -190,13 +192,13 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
         }
         if (lane == 0) {
             s_order = order;
-            s_at = (uint32_t)(begin - before);  // units of the sequence before the share
-            s_begin = units;
+            s_at = begin - before;  // units of the sequence before the share
+            s_units = units;
         }
     }
     if (!tab.step) pdl_enter();
     __syncthreads();
-    const uint64_t units = s_begin;
+    const uint64_t units = s_units;
     uint64_t pos = units * blockIdx.x / gridDim.x;
     const uint64_t end = units * (blockIdx.x + 1) / gridDim.x;
     uint32_t order = s_order;
@@ -211,15 +213,15 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
     // ---- row blocks, or the shares of them, one after another ---------------------------------------
     while (pos < end && order < tab.count) {
         const SeqRow seq = seq_load(tab, tab.ordered, order);
-        const uint32_t all_tiles = tiles_of(seq);
-        const uint64_t seq_units = (uint64_t)blocks_of(seq) * all_tiles;
+        const uint32_t all_units = units_of(seq);
+        const uint64_t seq_units = (uint64_t)blocks_of(seq) * all_units;
         if (at >= seq_units) {  // (an empty sequence, or the last one done)
             at = 0;
             order++;
             continue;
         }
-        const uint32_t block = (uint32_t)(at / all_tiles), first = (uint32_t)(at % all_tiles);
-        const uint32_t count = (uint32_t)min((uint64_t)(all_tiles - first), end - pos);
+        const uint32_t block = (uint32_t)(at / all_units), first = (uint32_t)(at % all_units);
+        const uint32_t count = (uint32_t)min((uint64_t)(all_units - first), end - pos);
         const uint64_t block_begin = pos - first;  // the row block's units on the line
         const int rows = (int)(seq.q_count * p.group), row0 = (int)block * R;  // score rows of the sequence; this block's first
         const int m_keys = (int)seq.k_count, shift = m_keys - (int)seq.q_count;
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
         const int tile_first = (int)(seq.k_start / 64);
         const int see_lo = (int)((seq.k_start + (uint32_t)b_lo) / 64) - tile_first;
         const int see_hi = b_hi > b_lo ? (int)(((uint64_t)seq.k_start + (uint32_t)b_hi + 63) / 64) - tile_first : see_lo;
-        const int tile0 = tile_first + max((int)first, see_lo), tile1 = tile_first + min((int)(first + count), see_hi);
+        const int tile0 = tile_first + max((int)first - kBlockCost, see_lo), tile1 = tile_first + min((int)(first + count) - kBlockCost, see_hi);
         const int tiles = tile1 - tile0;
         const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;  // tiles warp, warp + kWarps, ...
 
@@ -559,7 +561,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
             }
         }
         __syncthreads();
-        const bool whole_block = count == all_tiles;
+        const bool whole_block = count == all_units;
         // This share's place among the partial results: the first of the CTA's two if it begins with the CTA's
         // own share, else the second (a share is cut at its two ends only).
         const uint64_t begin = units * blockIdx.x / gridDim.x;
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
         }
         if (!whole_block) {
             // ---- the shares of a row block, merged by the CTA that finishes last --------------------------
-            const uint64_t block_end = block_begin + all_tiles;
+            const uint64_t block_end = block_begin + all_units;
             auto owner = [&](uint64_t unit) { return ((unit + 1) * gridDim.x - 1) / units; };  // the CTA a unit falls to
             const uint64_t cta0 = owner(block_begin), cta1 = owner(block_end - 1);
             const uint32_t shares = (uint32_t)(cta1 - cta0 + 1);
@@ -678,15 +680,15 @@ mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
     uint64_t units = 0, most = 0;  // now, and with a captured step's largest advance
     for (const SeqRow& r : a.host->rows) {
         const uint64_t blocks = ((uint64_t)r.q_count * p.group + R - 1) / R;
-        auto tiles = [&](uint64_t keys) { return std::max<uint64_t>(1, (r.k_start + keys + 63) / 64 - r.k_start / 64); };
+        auto tiles = [&](uint64_t keys) { return kBlockCost + (r.k_start + keys + 63) / 64 - r.k_start / 64; };
         units += blocks * tiles(r.k_count);
         most += blocks * tiles(r.k_count + a.max_step);
     }
     p.units = units;
     if (a.kv_head_count > 65535) return fail(MG_SHAPE_UNSUPPORTED, "attention kv_head_count exceeds the launch grid");
-    // One wave of CTAs, each with a tile at least for each of its warps.
+    // One wave of CTAs, each with a tile at least for each of its warps, beside a row block's cost.
     const uint64_t wave = std::max<uint64_t>(1, (uint64_t)d->sm_count * (NT == 1 ? kPerSm : 2) / a.kv_head_count);
-    const uint64_t shares = std::max<uint64_t>(1, std::min(wave, (most + kWarps - 1) / kWarps));
+    const uint64_t shares = std::max<uint64_t>(1, std::min(wave, (most + kBlockCost + kWarps - 1) / (kBlockCost + kWarps)));
     MG_TRY(scratch(d, 9, shares * a.kv_head_count * 2 * R * (D + 2) * sizeof(float), (void**)&p.partial));
     enqueue(d, attention_q4_kernel<T, D, NT>, dim3((unsigned)shares, (unsigned)a.kv_head_count), kThreads, S::kSmem, p);
     return launched(d, "4-bit attention launch");
