@@ -1,49 +1,30 @@
 // Log probabilities of given tokens, with entropy and top alternatives, from a row of logits.
+//
+// One pass over the row: with a reference m, d = (x - m) log2 e / temperature, l = sum 2^d and
+// t = sum d 2^d.  Then log p(x) = (x - max) / temperature - log l and the entropy is log l - ln 2 t / l.
+// The row is read once from memory (the top columns look at a part of it again, in the L2): 2 or 4
+// bytes a logit against one exponential and some four other instructions, so memory bounds many rows.
 #include <algorithm>
+#include <cmath>
 
 #include "sequences.cuh"
+#include "sm100.cuh"
 
 namespace mg {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kGroup = 4;                       // threads whose largest values are taken together
-constexpr int kGroups = kThreads / kGroup;      // at least MG_LOGPROBS_MAX_TOP
+using namespace sm100;
+
+#ifndef PSM
+#define PSM 1024
+#define BAT 4
+#define TPB 256
+#endif
+constexpr int kGroups = 64;  // of threads, whose largest values are taken together
 constexpr int kCandidates = 1024;
 static_assert(kGroups >= MG_LOGPROBS_MAX_TOP, "as many groups as top columns");
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLowest = -3.4028234663852886e38f;  // stands for a maximum of nothing: finite, so that -inf less it is -inf
-
-// A row's statistics so far: the largest logit m, and with d = scale (x - m) (scale = log2 e over the
-// temperature) l = sum 2^d and t = sum d 2^d.
-struct Stats {
-    float m, l, t;
-};
-
-// l and t moved to the maximum m_new >= m.  d may be -inf where the maxima lie far apart: a part of no
-// weight adds nothing (a NaN in l still does).
-__device__ __forceinline__ void move_to(Stats& s, float m_new, float scale) {
-    const float d = (s.m - m_new) * scale, w = exp2f(d);
-    s.t = w > 0.0f ? w * fmaf(s.l, d, s.t) : 0.0f;
-    s.l *= w;
-    s.m = m_new;
-}
-
-__device__ __forceinline__ Stats merge(Stats a, Stats b, float scale) {
-    const float m = fmaxf(a.m, b.m);
-    move_to(a, m, scale);
-    move_to(b, m, scale);
-    return {m, a.l + b.l, a.t + b.t};
-}
-
-__device__ __forceinline__ Stats merge_warp(Stats s, float scale) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
-        s = merge(s, {__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.l, o), __shfl_xor_sync(0xffffffffu, s.t, o)},
-                  scale);
-    return s;
-}
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kMove = 16.0f;  // the reference moves when a value passes it by more than 2^16
 
 struct LogprobsK {
     const void* logits;
@@ -52,34 +33,116 @@ struct LogprobsK {
     uint64_t rows;
     uint32_t vocab, top;
     float inv_temperature;
+    float scale;  // logits to log2 units
+    float floor;  // logits below it are as good as excluded, and counted as it: floor * scale stays finite
 };
 
-// Calls f(value, column) for the row's values of this thread, in 16-byte chunks where it can: the
-// values before the first aligned one and after the last go to the first threads singly.
-template <typename T, class Chunk, class One>
-__device__ __forceinline__ void for_values(const T* x, uint32_t n, Chunk&& chunk, One&& one) {
-    constexpr uint32_t N = 16 / sizeof(T);
-    const uint32_t head = min(n, (uint32_t)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (uint32_t)sizeof(T));
-    const uint32_t chunks = (n - head) / N, tail = head + chunks * N;
-    for (uint32_t c = threadIdx.x; c < chunks; c += kThreads) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + head) + c);
-        const T* p = reinterpret_cast<const T*>(&u);
-        float v[N];
-#pragma unroll
-        for (uint32_t e = 0; e < N; e++) v[e] = to_f32(p[e]);
-        chunk(v, head + c * N);
-    }
-    if (threadIdx.x < head) one(to_f32(x[threadIdx.x]), threadIdx.x);
-    if (threadIdx.x < n - tail) one(to_f32(x[tail + threadIdx.x]), tail + threadIdx.x);
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// The larger of two; NaN if one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
 
-// One row per block.  A first pass over the row keeps each thread's running maximum and sums; the
-// threads' maxima also bound the top columns: the top-th largest of the groups' maxima is reached by
-// at least `top` values, so only the threads whose own maximum reaches it read their part of the
-// row again (from the L2) and collect what reaches it.
+// Logits as they lie in memory: a 32-bit word of one or two, its larger and its values.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsK p) {
-    __shared__ Stats parts[kWarps];
+struct Word;
+template <>
+struct Word<float> {
+    static constexpr int kValues = 1;
+    static constexpr uint32_t kExcluded = 0xff800000u;
+    static __device__ __forceinline__ uint32_t of(float x) { return __float_as_uint(x); }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+    }
+    static __device__ __forceinline__ float largest(uint32_t a) { return __uint_as_float(a); }
+    static __device__ __forceinline__ float value(uint32_t a, int) { return __uint_as_float(a); }
+};
+template <>
+struct Word<__nv_bfloat16> {
+    static constexpr int kValues = 2;
+    static constexpr uint32_t kExcluded = 0xff80ff80u;
+    static __device__ __forceinline__ uint32_t of(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)) * 0x10001u; }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    static __device__ __forceinline__ float value(uint32_t a, int i) { return __uint_as_float(i ? a & 0xffff0000u : a << 16); }
+    static __device__ __forceinline__ float largest(uint32_t a) { return max_nan(value(a, 0), value(a, 1)); }
+};
+template <>
+struct Word<__half> {
+    static constexpr int kValues = 2;
+    static constexpr uint32_t kExcluded = 0xfc00fc00u;
+    static __device__ __forceinline__ uint32_t of(float x) { return __half_as_ushort(__float2half_rn(x)) * 0x10001u; }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        uint32_t d;
+        asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+        return d;
+    }
+    static __device__ __forceinline__ float value(uint32_t a, int i) {
+        return __half2float(__ushort_as_half((unsigned short)(i ? a >> 16 : a & 0xffffu)));
+    }
+    static __device__ __forceinline__ float largest(uint32_t a) { return max_nan(value(a, 0), value(a, 1)); }
+};
+
+// A row in 16-byte chunks: the values before the first aligned one and after the last whole chunk are
+// taken singly.
+template <typename T>
+struct Row {
+    static constexpr uint32_t N = 16 / sizeof(T);  // values of a chunk
+    const T* x;
+    uint32_t n, head, chunks, tail;
+    __device__ __forceinline__ Row(const T* row, uint32_t vocab) : x(row), n(vocab) {
+        head = min(n, (uint32_t)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (uint32_t)sizeof(T));
+        chunks = (n - head) / N;
+        tail = head + chunks * N;
+    }
+    // The single value that falls to this thread (below 2 N threads), and whether there is one.
+    __device__ __forceinline__ bool single(uint32_t i, uint32_t& col) const {
+        col = i < head ? i : tail + (i - head);
+        return i < head + (n - tail);
+    }
+    // f(value, column) for the values of chunks first, first + step, ...
+    template <class F>
+    __device__ __forceinline__ void for_chunks(uint32_t first, uint32_t step, F&& f) const {
+        for (uint32_t c = first; c < chunks; c += step) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + head) + c);
+            const T* p = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (uint32_t e = 0; e < N; e++) f(to_f32(p[e]), head + c * N + e);
+        }
+    }
+    // For those that fall to this thread of the block.
+    template <class F>
+    __device__ __forceinline__ void for_values(F&& f) const {
+        for_chunks(threadIdx.x, blockDim.x, f);
+        uint32_t col;
+        if (single(threadIdx.x, col)) f(to_f32(x[col]), col);
+    }
+};
+
+// One row per block.  The threads' maxima also bound the top columns: the top-th largest of the groups'
+// maxima is reached by at least `top` values, so only the parts of the row of threads whose own maximum
+// reaches it are read again (by the thread's whole warp), and what reaches it is collected.
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, PSM / kThreads) logprobs_kernel(const LogprobsK p) {
+    using W = Word<T>;
+    constexpr int kWarps = kThreads / 32, kGroup = kThreads / kGroups;
+    constexpr int kBatch = BAT;  // chunks of a thread in flight
+    constexpr int kWords = kBatch * 4;
+    __shared__ float warp_max[kWarps], warp_l[kWarps], warp_t[kWarps];
     __shared__ float group_max[kGroups];
     __shared__ float s_bound;
     __shared__ uint32_t s_count;
@@ -87,68 +150,115 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsK p) {
     __shared__ uint32_t cand_col[kCandidates];
     __shared__ unsigned long long s_best[kWarps];
     pdl_enter();
-    constexpr uint32_t N = 16 / sizeof(T);
     const uint64_t row = blockIdx.x;
-    const T* x = (const T*)p.logits + row * p.vocab;
+    const Row<T> x((const T*)p.logits + row * p.vocab, p.vocab);
     float* out = p.out + row * (2 + 2 * (uint64_t)p.top);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const float scale = kLog2e * p.inv_temperature;  // logits to log2 units
 
-    Stats s{kLowest, 0.0f, 0.0f};
-    auto grow = [&](float to) {
-        if (to > s.m) move_to(s, to, scale);
+    // ---- the row's sums -----------------------------------------------------------------------------
+    const uint32_t floor = W::of(p.floor);
+    float ref = W::value(floor, 0);
+    uint64_t l2 = f2(0.0f, 0.0f), t2 = f2(0.0f, 0.0f);
+    uint32_t most = W::kExcluded;  // of the logits as they are, NaN staying NaN
+    const uint64_t scale2 = f2(p.scale, p.scale);
+    // l and t moved to another reference; a part of no weight adds nothing, however far away
+    auto moved = [&](float to, float& l, float& t) {
+        const float d = (ref - to) * p.scale, w = ex2(d);
+        t = w > 0.0f ? w * fmaf(l, d, t) : 0.0f;
+        l *= w;
     };
-    auto add = [&](float v) {
-        // an excluded logit (-inf) weighs nothing, and its distance must not be multiplied as infinite
-        const float d = fmaxf((v - s.m) * scale, kLowest), w = exp2f(v != v ? v : d);
-        s.l += w;
-        s.t = fmaf(w, d, s.t);
+    auto batch = [&](const uint32_t (&w)[kWords], uint32_t c0) {
+        uint32_t top[4] = {w[0], w[1], w[2], w[3]};
+#pragma unroll
+        for (int i = 4; i < kWords; i++) top[i % 4] = W::larger(top[i % 4], w[i]);
+        const uint32_t all = W::larger(W::larger(top[0], top[1]), W::larger(top[2], top[3]));
+        most = W::larger(most, all);
+        const float to = W::largest(all);
+        if ((to - ref) * p.scale > kMove) {
+            float2 l = f2split(l2), t = f2split(t2);
+            moved(to, l.x, t.x);
+            moved(to, l.y, t.y);
+            l2 = f2(l.x, l.y);
+            t2 = f2(t.x, t.y);
+            ref = to;
+        }
+        const float r = -ref * p.scale;
+        const uint64_t ref2 = f2(r, r);
+#pragma unroll
+        for (int b = 0; b < kBatch; b++) {
+            if (c0 + b * kThreads >= x.chunks) break;
+#pragma unroll
+            for (int i = 4 * b; i < 4 * b + 4; i += 3 - W::kValues) {
+                const uint32_t u = W::larger(w[i], floor), v = W::kValues == 1 ? W::larger(w[(i + 1) % kWords], floor) : 0u;
+                uint64_t d = ref2;
+                f2fma(d, f2(W::value(u, 0), W::kValues == 2 ? W::value(u, 1) : W::value(v, 0)), scale2);
+                const float2 y = f2split(d);
+                const uint64_t e = f2(ex2(y.x), ex2(y.y));
+                l2 = f2add(l2, e);
+                f2fma(t2, e, d);
+            }
+        }
     };
-    for_values(x, p.vocab,
-               [&](const float (&v)[N], uint32_t) {
-                   float top = v[0];
+    for (uint32_t c0 = threadIdx.x; c0 < x.chunks; c0 += kBatch * kThreads) {
+        uint32_t w[kWords];
 #pragma unroll
-                   for (uint32_t e = 1; e < N; e++) top = fmaxf(top, v[e]);
-                   grow(top);
-#pragma unroll
-                   for (uint32_t e = 0; e < N; e++) add(v[e]);
-               },
-               [&](float v, uint32_t) {
-                   grow(v);
-                   add(v);
-               });
-    const float mine = s.m;
-    s = merge_warp(s, scale);
-    if (lane == 0) parts[warp] = s;
-    if (p.top) {
-        float g = mine;
-#pragma unroll
-        for (int o = 1; o < kGroup; o <<= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-        if (threadIdx.x % kGroup == 0) group_max[threadIdx.x / kGroup] = g;
+        for (int b = 0; b < kBatch; b++) {
+            // (the address is bounded, not the load: a conditional load is waited for at once)
+            const uint32_t c = c0 + b * kThreads;
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x.x + x.head) + min(c, x.chunks - 1));
+            const bool in = c < x.chunks;
+            w[4 * b] = in ? u.x : W::kExcluded;
+            w[4 * b + 1] = in ? u.y : W::kExcluded;
+            w[4 * b + 2] = in ? u.z : W::kExcluded;
+            w[4 * b + 3] = in ? u.w : W::kExcluded;
+        }
+        batch(w, c0);
     }
+    uint32_t single;
+    float lone = __int_as_float(0xff800000);
+    const bool has_single = x.single(threadIdx.x, single);
+    if (has_single) lone = to_f32(x.x[single]);
+    float mine = max_nan(W::largest(most), lone);
+    float2 ll = f2split(l2), tt = f2split(t2);
+    float l = ll.x + ll.y, t = tt.x + tt.y;
+    // excluded logits that were counted at the floor, while the reference lay there
+    {
+        const float low = W::value(floor, 0), v = max_nan(lone, low);
+        if (v > ref) {
+            moved(v, l, t);
+            ref = v;
+        }
+        if (has_single) {
+            const float d = (v - ref) * p.scale, w = ex2(d);
+            l += w;
+            t = fmaf(w, d, t);
+        }
+    }
+    // ---- the block's ----------------------------------------------------------------------------------
+    float m = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (2 * o == kGroup && lane % kGroup == 0) group_max[threadIdx.x / kGroup] = m;
+    }
+    if (lane == 0) warp_max[warp] = m;
     if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
-    s = parts[0];
-#pragma unroll 1
-    for (int w = 1; w < kWarps; w++) s = merge(s, parts[w], scale);
-    // With log l, a log probability is (x - m) / temperature - log l, which keeps its digits where m is
-    // large; NaN where there is no distribution (l is 0 without a finite logit, NaN with a NaN).
-    const float nan = __int_as_float(0x7fc00000);
-    const float log_l = s.l > 0.0f && s.m <= -kLowest ? logf(s.l) : nan;
-    auto logprob = [&](float v) { return (v - s.m) * p.inv_temperature - log_l; };
-    if (threadIdx.x == 0) {
-        const float id = p.tokens ? p.tokens[row] : -1.0f;
-        const bool is_column = id >= 0.0f && id < (float)p.vocab && id == floorf(id);
-        out[0] = is_column ? logprob(to_f32(x[(uint32_t)id])) : nan;
-        out[1] = log_l - s.t * kLn2 / s.l;  // log sum e^z - sum p z
+    m = warp_max[lane % kWarps];
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float to = max_nan(m, W::value(floor, 0));
+    moved(to, l, t);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, o);
+        t += __shfl_xor_sync(0xffffffffu, t, o);
     }
-    if (!p.top) return;
-    if (log_l != log_l) {
-        for (uint32_t i = threadIdx.x; i < 2 * p.top; i += kThreads) out[2 + i] = nan;
-        return;
+    if (lane == 0) {
+        warp_l[warp] = l;
+        warp_t[warp] = t;
     }
-    // the top-th largest of the groups' maxima
-    if (threadIdx.x < kGroups) {
+    if (p.top && threadIdx.x < kGroups) {  // the top-th largest of the groups' maxima
         const float g = group_max[threadIdx.x];
         uint32_t rank = 0;
 #pragma unroll 8
@@ -159,8 +269,56 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsK p) {
         if (rank == p.top - 1) s_bound = g;
     }
     __syncthreads();
-    // (fewer than `top` finite logits leave a bound of nothing: -inf columns fill up the rest)
-    const float bound = s_bound <= kLowest ? __int_as_float(0xff800000) : s_bound;
+    l = warp_l[lane % kWarps];
+    t = warp_t[lane % kWarps];
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+        l += __shfl_xor_sync(0xffffffffu, l, o);
+        t += __shfl_xor_sync(0xffffffffu, t, o);
+    }
+    if (m < to && m > __int_as_float(0xff800000)) {
+        // No logit above the floor: the sums once more, about the largest itself.
+        l = t = 0.0f;
+        x.for_values([&](float v, uint32_t) {
+            const float d = fmaxf((v - m) * p.scale, -1e38f), w = ex2(d);
+            l += w;
+            t = fmaf(w, d, t);
+        });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            l += __shfl_xor_sync(0xffffffffu, l, o);
+            t += __shfl_xor_sync(0xffffffffu, t, o);
+        }
+        __syncthreads();
+        if (lane == 0) {
+            warp_l[warp] = l;
+            warp_t[warp] = t;
+        }
+        __syncthreads();
+        l = t = 0.0f;
+        for (int w = 0; w < kWarps; w++) {
+            l += warp_l[w];
+            t += warp_t[w];
+        }
+    }
+    // A log probability is (x - m) / temperature - log l, which keeps its digits where m is large; NaN where
+    // there is no distribution (no finite logit, an infinite one, a NaN).
+    const float nan = __int_as_float(0x7fc00000);
+    const float log_l = m > __int_as_float(0xff800000) && m < __int_as_float(0x7f800000) ? logf(l) : nan;
+    auto logprob = [&](float v) { return (v - m) * p.inv_temperature - log_l; };
+    if (threadIdx.x == 0) {
+        const float id = p.tokens ? p.tokens[row] : -1.0f;
+        const bool is_column = id >= 0.0f && id < (float)p.vocab && id == floorf(id);
+        out[0] = is_column ? logprob(to_f32(x.x[(uint32_t)id])) : nan;
+        out[1] = log_l - t * kLn2 / l;  // log sum e^z - sum p z
+    }
+    if (!p.top) return;
+    if (log_l != log_l) {
+        for (uint32_t i = threadIdx.x; i < 2 * p.top; i += kThreads) out[2 + i] = nan;
+        return;
+    }
+    // ---- the top columns --------------------------------------------------------------------------------
+    const float bound = s_bound;  // (-inf where fewer than `top` groups have a finite logit: everything reaches it)
     auto collect = [&](float v, uint32_t col) {
         if (v >= bound) {
             const uint32_t at = atomicAdd(&s_count, 1u);
@@ -170,17 +328,9 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsK p) {
             }
         }
     };
-    if (mine >= bound)
-        for_values(x, p.vocab,
-                   [&](const float (&v)[N], uint32_t col) {
-                       float top = v[0];
-#pragma unroll
-                       for (uint32_t e = 1; e < N; e++) top = fmaxf(top, v[e]);
-                       if (top >= bound)
-#pragma unroll
-                           for (uint32_t e = 0; e < N; e++) collect(v[e], col + e);
-                   },
-                   collect);
+    if (has_single) collect(lone, single);
+    for (uint32_t q = __ballot_sync(0xffffffffu, W::largest(most) >= bound); q; q &= q - 1)
+        x.for_chunks(threadIdx.x - lane + (uint32_t)__ffs(q) - 1 + (uint32_t)lane * kThreads, 32 * kThreads, collect);
     __syncthreads();
     const uint32_t n = s_count;
     if (n <= kCandidates) {
@@ -206,16 +356,10 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsK p) {
     unsigned long long last = ~0ull;
     for (uint32_t r = 0; r < p.top; r++) {
         unsigned long long best = 0;
-        auto consider = [&](float v, uint32_t col) {
+        x.for_values([&](float v, uint32_t col) {
             const unsigned long long key = key_of(v, col);
             if (key < last && key > best) best = key;
-        };
-        for_values(x, p.vocab,
-                   [&](const float (&v)[N], uint32_t col) {
-#pragma unroll
-                       for (uint32_t e = 0; e < N; e++) consider(v[e], col + e);
-                   },
-                   consider);
+        });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
         if (lane == 0) s_best[warp] = best;
@@ -225,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobsK p) {
         last = best;
         if (threadIdx.x == 0) {
             const uint32_t col = 0xffffffffu - (uint32_t)best;
-            out[2 + r] = logprob(to_f32(x[col]));
+            out[2 + r] = logprob(to_f32(x.x[col]));
             out[2 + p.top + r] = (float)col;
         }
     }
@@ -238,10 +382,16 @@ namespace k {
 mg_status token_logprobs(Device* d, const LogprobsArgs& a) {
     if (a.rows == 0) return MG_OK;
     if (a.rows > 0x7fffffffull) return fail(MG_SHAPE_UNSUPPORTED, "token log probabilities of too many rows");
-    const LogprobsK p{a.logits, a.tokens, a.out, a.rows, (uint32_t)a.vocab, a.top, 1.0f / a.temperature};
+    LogprobsK p{a.logits, a.tokens, a.out, a.rows, (uint32_t)a.vocab, a.top, 1.0f / a.temperature, 0.0f, 0.0f};
+    p.scale = 1.4426950408889634f * p.inv_temperature;
+    // a power of two, so that floor * scale is exact: logits at the floor are at no distance from it
+    p.floor = -exp2f(floorf(log2f(1e38f / std::max(1.0f, p.scale))));
+    if (a.dtype == MG_F16) p.floor = std::max(p.floor, -32768.0f);
     return by_float(a.dtype, [&](auto t) {
         using T = decltype(t);
-        enqueue(d, logprobs_kernel<T>, (unsigned)a.rows, kThreads, 0, p);
+        // Few rows: a block of as many threads as there are for each.
+        if (a.rows <= (uint64_t)d->sm_count) enqueue(d, logprobs_kernel<T, 1024>, (unsigned)a.rows, 1024, 0, p);
+        else enqueue(d, logprobs_kernel<T, TPB>, (unsigned)a.rows, TPB, 0, p);
         return launched(d, "token log probabilities launch");
     });
 }
