@@ -26,32 +26,14 @@ __device__ __forceinline__ uint8_t* record(void* store, uint64_t row, uint64_t c
     return (uint8_t*)store + (row / kQ4Tile * columns + column) * kQ4Record;
 }
 
-// A thread's places in packed rows of `columns` pieces each, kStride pieces apart: one division at the
-// start, then additions (a division by a variable is some 20 instructions, of 64 bits 70).
+// A thread's places in packed rows, and the store rows they belong to.
 template <uint32_t kStride>
-struct Walk {
-    uint64_t i, advance;
-    uint32_t c, step_rows, step_columns, columns;
+struct Walk : Places<kStride> {
+    using Places<kStride>::i;
+    uint64_t advance;
     SeqRow s{0, 0, 0, 0};
-    __device__ __forceinline__ Walk(const k::KvPackedArgs& a, uint64_t first, uint32_t columns_) : columns(columns_) {
-        if (first >> 32) {
-            i = first / columns;
-            c = (uint32_t)(first % columns);
-        } else {
-            i = (uint32_t)first / columns;
-            c = (uint32_t)first % columns;
-        }
-        step_rows = kStride / columns;
-        step_columns = kStride % columns;
+    __device__ __forceinline__ Walk(const k::KvPackedArgs& a, uint64_t first, uint32_t columns) : Places<kStride>(first, columns) {
         advance = a.row_offset + (a.table.count == 0 && a.table.step ? *a.table.step : 0);
-    }
-    __device__ __forceinline__ void next() {
-        i += step_rows;
-        c += step_columns;
-        if (c >= columns) {
-            c -= columns;
-            i++;
-        }
     }
     // The store row that packed row i goes to (or is read from).
     __device__ __forceinline__ uint64_t row(const k::KvPackedArgs& a) {

@@ -39,6 +39,33 @@ __device__ __forceinline__ uint32_t seq_of_query(const k::SeqTable& t, uint32_t 
     return lo;
 }
 
+// A thread's places in rows of `columns` pieces each, kStride pieces apart: one division at the start, then
+// additions (a division by a variable is some 20 instructions, of 64 bits 70).
+template <uint32_t kStride>
+struct Places {
+    uint64_t i;                                    // row
+    uint32_t c, step_rows, step_columns, columns;  // piece of the row; the stride
+    __device__ __forceinline__ Places(uint64_t first, uint32_t columns_) : columns(columns_) {
+        if (first >> 32) {
+            i = first / columns;
+            c = (uint32_t)(first % columns);
+        } else {
+            i = (uint32_t)first / columns;
+            c = (uint32_t)first % columns;
+        }
+        step_rows = kStride / columns;
+        step_columns = kStride % columns;
+    }
+    __device__ __forceinline__ void next() {
+        i += step_rows;
+        c += step_columns;
+        if (c >= columns) {
+            c -= columns;
+            i++;
+        }
+    }
+};
+
 // Work item `item` of a launch that gives a sequence of n queries `items_of(n)` items, sequences with the
 // most keys first: the sequence's place in that order and the item's place in the sequence.  All lanes of
 // a warp call it together; false past the last item.
