@@ -3,7 +3,7 @@
 // One pass over the row: with a reference m, d = (x - m) log2 e / temperature, l = sum 2^d and
 // t = sum d 2^d.  Then log p(x) = (x - max) / temperature - log l and the entropy is log l - ln 2 t / l.
 // The row is read once from memory (the top columns look at a part of it again, in the L2): 2 or 4
-// bytes a logit against one exponential and some four other instructions, so memory bounds many rows.
+// bytes a logit against one exponential and some six other instructions.
 #include <algorithm>
 #include <cmath>
 
@@ -16,10 +16,11 @@ namespace {
 using namespace sm100;
 
 // Threads of an SM, of a block (where there are more rows than SMs), and 16-byte chunks of a thread in
-// flight.  8192 rows of 32000 bf16: 138 us; 1024 threads an SM 163, blocks of 128 threads 150 to 240,
-// 2 chunks 149 (the 40 registers of 1536 threads just hold 4).
+// flight.  8192 rows of 32000 bf16: 132 us, 4.0 TB/s, bound by instruction issue (two thirds of the slots,
+// half of the exponentials' unit); 1280 threads an SM 136, blocks of 128 threads 139 and of 512 172, 2 chunks
+// 138 (the 40 registers of 1536 threads just hold 4).
 constexpr int kPerSm = 1536, kBlock = 256, kBatch = 4;
-constexpr int kGroups = 64;  // of threads, whose largest values are taken together
+constexpr int kGroups = 64;  // at the most, of threads whose largest values are taken together
 constexpr int kCandidates = 1024;
 static_assert(kGroups >= MG_LOGPROBS_MAX_TOP, "as many groups as top columns");
 constexpr float kLn2 = 0.6931471805599453f;
@@ -113,20 +114,15 @@ struct Row {
         col = i < head ? i : tail + (i - head);
         return i < head + (n - tail);
     }
-    // f(value, column) for the values of chunks first, first + step, ...
+    // f(value, column) for those that fall to this thread of the block.
     template <class F>
-    __device__ __forceinline__ void for_chunks(uint32_t first, uint32_t step, F&& f) const {
-        for (uint32_t c = first; c < chunks; c += step) {
+    __device__ __forceinline__ void for_values(F&& f) const {
+        for (uint32_t c = threadIdx.x; c < chunks; c += blockDim.x) {
             const uint4 u = __ldg(reinterpret_cast<const uint4*>(x + head) + c);
             const T* p = reinterpret_cast<const T*>(&u);
 #pragma unroll
             for (uint32_t e = 0; e < N; e++) f(to_f32(p[e]), head + c * N + e);
         }
-    }
-    // For those that fall to this thread of the block.
-    template <class F>
-    __device__ __forceinline__ void for_values(F&& f) const {
-        for_chunks(threadIdx.x, blockDim.x, f);
         uint32_t col;
         if (single(threadIdx.x, col)) f(to_f32(x[col]), col);
     }
@@ -138,7 +134,7 @@ struct Row {
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(const LogprobsK p) {
     using W = Word<T>;
-    constexpr int kWarps = kThreads / 32, kGroup = kThreads / kGroups;
+    constexpr int kWarps = kThreads / 32;
     constexpr int kWords = kBatch * 4;
     __shared__ float warp_max[kWarps], warp_l[kWarps], warp_t[kWarps];
     __shared__ float group_max[kGroups];
@@ -165,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         t = w > 0.0f ? w * fmaf(l, d, t) : 0.0f;
         l *= w;
     };
-    auto batch = [&](const uint32_t (&w)[kWords], uint32_t c0) {
+    // (a thread's batch holds n chunks; the rest of w is excluded logits)
+    auto batch = [&](const uint32_t (&w)[kWords], int n) {
         uint32_t top[4] = {w[0], w[1], w[2], w[3]};
 #pragma unroll
         for (int i = 4; i < kWords; i++) top[i % 4] = W::larger(top[i % 4], w[i]);
@@ -184,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         const uint64_t ref2 = f2(r, r);
 #pragma unroll
         for (int b = 0; b < kBatch; b++) {
-            if (c0 + b * kThreads >= x.chunks) break;
+            if (b >= n) break;
 #pragma unroll
             for (int i = 4 * b; i < 4 * b + 4; i += 3 - W::kValues) {
                 const uint32_t u = W::larger(w[i], floor), v = W::kValues == 1 ? W::larger(w[(i + 1) % kWords], floor) : 0u;
@@ -197,20 +194,32 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
             }
         }
     };
-    for (uint32_t c0 = threadIdx.x; c0 < x.chunks; c0 += kBatch * kThreads) {
+    const uint4* chunk = reinterpret_cast<const uint4*>(x.x + x.head) + threadIdx.x;
+    int left = x.chunks > threadIdx.x ? (int)((x.chunks - threadIdx.x + kThreads - 1) / kThreads) : 0;  // of this thread
+    for (; left >= kBatch; left -= kBatch, chunk += kBatch * kThreads) {
+        uint32_t w[kWords];
+#pragma unroll
+        for (int b = 0; b < kBatch; b++) {
+            const uint4 u = __ldg(chunk + b * kThreads);
+            w[4 * b] = u.x;
+            w[4 * b + 1] = u.y;
+            w[4 * b + 2] = u.z;
+            w[4 * b + 3] = u.w;
+        }
+        batch(w, kBatch);
+    }
+    if (left) {
         uint32_t w[kWords];
 #pragma unroll
         for (int b = 0; b < kBatch; b++) {
             // (the address is bounded, not the load: a conditional load is waited for at once)
-            const uint32_t c = c0 + b * kThreads;
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x.x + x.head) + min(c, x.chunks - 1));
-            const bool in = c < x.chunks;
-            w[4 * b] = in ? u.x : W::kExcluded;
-            w[4 * b + 1] = in ? u.y : W::kExcluded;
-            w[4 * b + 2] = in ? u.z : W::kExcluded;
-            w[4 * b + 3] = in ? u.w : W::kExcluded;
+            const uint4 u = __ldg(chunk + min(b, left - 1) * kThreads);
+            w[4 * b] = b < left ? u.x : W::kExcluded;
+            w[4 * b + 1] = b < left ? u.y : W::kExcluded;
+            w[4 * b + 2] = b < left ? u.z : W::kExcluded;
+            w[4 * b + 3] = b < left ? u.w : W::kExcluded;
         }
-        batch(w, c0);
+        batch(w, left);
     }
     uint32_t single;
     float lone = __int_as_float(0xff800000);
@@ -233,11 +242,13 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         }
     }
     // ---- the block's ----------------------------------------------------------------------------------
+    // (half the groups where they are enough: half the comparisons below for a few more candidates)
+    const int groups = p.top <= kGroups / 2 ? kGroups / 2 : kGroups, group = kThreads / groups;
     float m = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (2 * o == kGroup && lane % kGroup == 0) group_max[threadIdx.x / kGroup] = m;
+        if (2 * o == group && lane % group == 0) group_max[threadIdx.x / group] = m;
     }
     if (lane == 0) warp_max[warp] = m;
     if (threadIdx.x == 0) s_count = 0;
@@ -256,11 +267,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         warp_l[warp] = l;
         warp_t[warp] = t;
     }
-    if (p.top && threadIdx.x < kGroups) {  // the top-th largest of the groups' maxima
+    if (p.top && threadIdx.x < groups) {  // the top-th largest of the groups' maxima
         const float g = group_max[threadIdx.x];
         uint32_t rank = 0;
 #pragma unroll 8
-        for (int i = 0; i < kGroups; i++) {
+        for (int i = 0; i < groups; i++) {
             const float o = group_max[i];
             rank += o > g || (o == g && i < (int)threadIdx.x);
         }
@@ -327,8 +338,24 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         }
     };
     if (has_single) collect(lone, single);
-    for (uint32_t q = __ballot_sync(0xffffffffu, W::largest(most) >= bound); q; q &= q - 1)
-        x.for_chunks(threadIdx.x - lane + (uint32_t)__ffs(q) - 1 + (uint32_t)lane * kThreads, 32 * kThreads, collect);
+    // (chunks of one thread at a time, or of two where a half warp covers them)
+    const bool two = x.chunks <= 16u * kThreads;
+    for (uint32_t q = __ballot_sync(0xffffffffu, W::largest(most) >= bound); q; q &= q - 1) {
+        uint32_t of = (uint32_t)__ffs(q) - 1, at = lane;
+        if (two) {
+            const uint32_t next = q & (q - 1);
+            at = lane & 15;
+            if (lane >= 16) of = next ? (uint32_t)__ffs(next) - 1 : 0xffffffu;
+            if (next) q = next;
+        }
+        for (uint32_t c = threadIdx.x - lane + of + at * kThreads; c < x.chunks; c += 32 * kThreads) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x.x + x.head) + c);
+            if (!(W::largest(W::larger(W::larger(u.x, u.y), W::larger(u.z, u.w))) >= bound)) continue;
+            const T* v = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (uint32_t e = 0; e < x.N; e++) collect(to_f32(v[e]), x.head + c * x.N + e);
+        }
+    }
     __syncthreads();
     const uint32_t n = s_count;
     if (n <= kCandidates) {
