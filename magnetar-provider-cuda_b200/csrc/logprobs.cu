@@ -20,8 +20,8 @@ using namespace sm100;
 // half of the exponentials' unit); 1280 threads an SM 136, blocks of 128 threads 139 and of 512 172, 2 chunks
 // 138 (the 40 registers of 1536 threads just hold 4).
 constexpr int kPerSm = 1536, kBlock = 256, kBatch = 4;
-constexpr int kGroups = 64;  // at the most, of threads whose largest values are taken together
-constexpr int kCandidates = 1024;
+constexpr int kGroups = 64;  // at the most, of threads whose largest values are taken together: 32 or 64
+constexpr int kCandidates = 512;
 static_assert(kGroups >= MG_LOGPROBS_MAX_TOP, "as many groups as top columns");
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMove = 16.0f;  // the reference moves when a value passes it by more than 2^16
@@ -137,12 +137,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
     constexpr int kWarps = kThreads / 32;
     constexpr int kWords = kBatch * 4;
     __shared__ float warp_max[kWarps], warp_l[kWarps], warp_t[kWarps];
+    __shared__ float lane_max[kWarps][32];
     __shared__ float group_max[kGroups];
     __shared__ float s_bound;
     __shared__ uint32_t s_count;
     __shared__ float cand[kCandidates];
     __shared__ uint32_t cand_col[kCandidates];
     __shared__ unsigned long long s_best[kWarps];
+    __shared__ uint32_t s_equal[kWarps];
     pdl_enter();
     const uint64_t row = blockIdx.x;
     const Row<T> x((const T*)p.logits + row * p.vocab, p.vocab);
@@ -242,14 +244,10 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         }
     }
     // ---- the block's ----------------------------------------------------------------------------------
-    // (half the groups where they are enough: half the comparisons below for a few more candidates)
-    const int groups = p.top <= kGroups / 2 ? kGroups / 2 : kGroups, group = kThreads / groups;
     float m = mine;
+    lane_max[warp][lane] = m;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (2 * o == group && lane % group == 0) group_max[threadIdx.x / group] = m;
-    }
+    for (int o = 1; o < 32; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
     if (lane == 0) warp_max[warp] = m;
     if (threadIdx.x == 0) s_count = 0;
     __syncthreads();
@@ -267,8 +265,17 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         warp_l[warp] = l;
         warp_t[warp] = t;
     }
-    if (p.top && threadIdx.x < groups) {  // the top-th largest of the groups' maxima
-        const float g = group_max[threadIdx.x];
+    // The top-th largest of the groups' maxima.  A group is a lane of all warps, or of every other one (a short
+    // row, which only the first warps read, still has all groups); the fewer groups where they are enough.
+    const int groups = p.top <= 32 ? 32 : 64;
+    float g = __int_as_float(0xff800000);
+    if (p.top && threadIdx.x < groups) {
+        for (int w = warp; w < kWarps; w += groups / 32) g = fmaxf(g, lane_max[w][lane]);
+        group_max[threadIdx.x] = g;
+    }
+    if (groups == 64) __syncthreads();
+    else __syncwarp();
+    if (p.top && threadIdx.x < groups) {
         uint32_t rank = 0;
 #pragma unroll 8
         for (int i = 0; i < groups; i++) {
@@ -327,37 +334,49 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         return;
     }
     // ---- the top columns --------------------------------------------------------------------------------
-    const float bound = s_bound;  // (-inf where fewer than `top` groups have a finite logit: everything reaches it)
-    auto collect = [&](float v, uint32_t col) {
-        if (v >= bound) {
-            const uint32_t at = atomicAdd(&s_count, 1u);
-            if (at < kCandidates) {
-                cand[at] = v;
-                cand_col[at] = col;
+    // (the bound is -inf where fewer than `top` groups have a finite logit)
+    const float bound = s_bound;
+    // Chunks of one thread at a time, or of two where a half warp covers them.  Where too many reach the bound
+    // (a mask that leaves few columns, many equal logits) once more for those above it.
+    const bool two = x.chunks <= 16u * kThreads;
+    uint32_t n = 0;
+    bool above = false;
+    for (;;) {
+        auto collect = [&](float v, uint32_t col) {
+            if (above ? v > bound : v >= bound) {
+                const uint32_t at = atomicAdd(&s_count, 1u);
+                if (at < kCandidates) {
+                    cand[at] = v;
+                    cand_col[at] = col;
+                }
+            }
+        };
+        if (has_single) collect(lone, single);
+        const float own = W::largest(most);
+        for (uint32_t q = __ballot_sync(0xffffffffu, above ? own > bound : own >= bound); q; q &= q - 1) {
+            uint32_t of = (uint32_t)__ffs(q) - 1, at = lane;
+            if (two) {
+                const uint32_t next = q & (q - 1);
+                at = lane & 15;
+                if (lane >= 16) of = next ? (uint32_t)__ffs(next) - 1 : 0xffffffu;
+                if (next) q = next;
+            }
+            for (uint32_t c = threadIdx.x - lane + of + at * kThreads; c < x.chunks; c += 32 * kThreads) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(x.x + x.head) + c);
+                if (!(W::largest(W::larger(W::larger(u.x, u.y), W::larger(u.z, u.w))) >= bound)) continue;
+                const T* v = reinterpret_cast<const T*>(&u);
+#pragma unroll
+                for (uint32_t e = 0; e < x.N; e++) collect(to_f32(v[e]), x.head + c * x.N + e);
             }
         }
-    };
-    if (has_single) collect(lone, single);
-    // (chunks of one thread at a time, or of two where a half warp covers them)
-    const bool two = x.chunks <= 16u * kThreads;
-    for (uint32_t q = __ballot_sync(0xffffffffu, W::largest(most) >= bound); q; q &= q - 1) {
-        uint32_t of = (uint32_t)__ffs(q) - 1, at = lane;
-        if (two) {
-            const uint32_t next = q & (q - 1);
-            at = lane & 15;
-            if (lane >= 16) of = next ? (uint32_t)__ffs(next) - 1 : 0xffffffu;
-            if (next) q = next;
-        }
-        for (uint32_t c = threadIdx.x - lane + of + at * kThreads; c < x.chunks; c += 32 * kThreads) {
-            const uint4 u = __ldg(reinterpret_cast<const uint4*>(x.x + x.head) + c);
-            if (!(W::largest(W::larger(W::larger(u.x, u.y), W::larger(u.z, u.w))) >= bound)) continue;
-            const T* v = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (uint32_t e = 0; e < x.N; e++) collect(to_f32(v[e]), x.head + c * x.N + e);
-        }
+        __syncthreads();
+        n = s_count;
+        if (n <= kCandidates || above) break;
+        __syncthreads();
+        if (threadIdx.x == 0) s_count = 0;
+        above = true;
+        __syncthreads();
     }
-    __syncthreads();
-    const uint32_t n = s_count;
     if (n <= kCandidates) {
         // each candidate's rank among them, ties by column
         for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
@@ -370,9 +389,27 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
                 out[2 + p.top + rank] = (float)col;
             }
         }
+        // the places that those above the bound leave: its first columns
+        for (uint32_t col0 = 0; n < p.top && col0 < p.vocab; col0 += kThreads) {
+            const uint32_t col = col0 + threadIdx.x;
+            const bool equal = col < p.vocab && to_f32(x.x[min(col, p.vocab - 1)]) == bound;
+            const uint32_t lanes = __ballot_sync(0xffffffffu, equal);
+            if (lane == 0) s_equal[warp] = (uint32_t)__popc(lanes);
+            __syncthreads();
+            uint32_t place = n + (uint32_t)__popc(lanes & ((1u << lane) - 1));
+            for (int w = 0; w < kWarps; w++) {
+                if (w < warp) place += s_equal[w];
+                n += s_equal[w];
+            }
+            if (equal && place < p.top) {
+                out[2 + place] = logprob(bound);
+                out[2 + p.top + place] = (float)col;
+            }
+            __syncthreads();
+        }
         return;
     }
-    // Very many equal logits: the largest (value, lowest column) below the last one taken, `top` times.
+    // Very many logits in very few groups: the largest (value, lowest column) below the last one taken, `top` times.
     // A key orders them: the value's bits made monotone (-0 as +0), then the column's complement.
     auto key_of = [](float v, uint32_t col) {
         const uint32_t b = __float_as_uint(v + 0.0f);
@@ -414,8 +451,9 @@ mg_status token_logprobs(Device* d, const LogprobsArgs& a) {
     if (a.dtype == MG_F16) p.floor = std::max(p.floor, -32768.0f);
     return by_float(a.dtype, [&](auto t) {
         using T = decltype(t);
-        // Few rows: a block of as many threads as there are for each.
-        if (a.rows <= (uint64_t)d->sm_count) enqueue(d, logprobs_kernel<T, 1024>, (unsigned)a.rows, 1024, 0, p);
+        // A block of 1024 threads where the rows leave SMs free and are long enough: 8 and 148 rows of 128 KB
+        // 5.3 and 7.5 us (of 256 threads 6.4 and 10.4), of 32 KB 4.3 and 4.9 (3.9 and 4.5).
+        if (a.rows <= (uint64_t)d->sm_count && a.vocab * sizeof(T) >= 49152) enqueue(d, logprobs_kernel<T, 1024>, (unsigned)a.rows, 1024, 0, p);
         else enqueue(d, logprobs_kernel<T, kBlock>, (unsigned)a.rows, kBlock, 0, p);
         return launched(d, "token log probabilities launch");
     });

@@ -445,6 +445,26 @@ def test_token_logprobs_ties_and_rows_without_a_distribution(kernels):
     assert got[7].tolist() == pytest.approx(got[0].tolist(), abs=1e-5)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows", [4, 200])
+@pytest.mark.parametrize("vocab,top", [(70, 64), (1024, 5), (32000, 20), (32000, 64)])
+def test_token_logprobs_of_few_allowed_columns(kernels, dtype, rows, vocab, top):
+    """A mask (-inf, or the type's lowest value) that leaves three columns, fewer than the top; a row of one value;
+    a row whose finite logits are all in every 256th column: columns of equal logits come in order."""
+    x = torch.full((rows, vocab), -math.inf, dtype=DT[dtype], device="cuda")
+    x[1] = torch.finfo(DT[dtype]).min
+    x[:, [5, vocab // 2, vocab - 1]] = randn((rows, 3), dtype, 75)
+    x[2] = 0.5
+    x[3, ::256] = randn((vocab + 255) // 256, dtype, 76)
+    torch.cuda.synchronize()
+    got = to_torch(kernels, kernels.token_logprobs(kernels.wrap_tensor(x), None, top=top))
+    want = logprobs64(x, torch.full((rows,), -1.0, device="cuda"), top, 1.0)
+    assert torch.equal(got[:, 2 + top:].double(), want[:, 2 + top:])
+    finite = torch.isfinite(want[:, 1:2 + top]) & (want[:, 1:2 + top].abs() < 1e30)
+    assert torch.equal(got[:, 1:2 + top][~finite].double(), want[:, 1:2 + top][~finite].float().double())
+    assert float((got[:, 1:2 + top].double() - want[:, 1:2 + top])[finite].abs().max()) <= 1e-5
+
+
 def test_token_logprobs_rows_on_odd_addresses(kernels):
     x = randn((1 + 3 * 1001,), "bf16", 71)[1:].view(3, 1001)
     tokens = torch.tensor([0.0, 1000.0, 500.5], device="cuda")
