@@ -5,37 +5,89 @@
 // keys up to and with that position, a window of w the last w of those.  A query that sees no key
 // gives zeros.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention_packed.cuh"
 
 namespace mg {
 namespace {
 
-// Any dimensions up to 512, any alignment: one warp per (query, head).
-constexpr int kRowThreads = 256;
+// Any dimensions up to 512, any alignment, on the CUDA cores: one warp per (query, head), or SPLIT: a block for
+// each, whose warps take every eighth 32 keys and are merged at the end.
+// Four prompts of up to 512 tokens, 16 heads over 4 of 96, bfloat16: 0.42 ms (keys one at a time by lanes over the
+// dimensions, as this kernel once did: 5.8); one query each of four over 64 to 3000 keys: 58 us (one warp each:
+// 0.85 ms).  Bound by the loads' latency: a key's row is 16-byte pieces of 32 different lines.
+constexpr int kRowWarps = 8, kRowThreads = 32 * kRowWarps;
+
+template <typename T, typename R, int N, bool SPLIT>
+__global__ void __launch_bounds__(kRowThreads) attention_packed_row_kernel(const k::PackedAttentionArgs a, R kr, R vr) {
+    __shared__ __align__(16) float q_shared[kRowWarps][k::kPackedMaxDim];
+    __shared__ float means[SPLIT ? kRowWarps : 1][32 * N];
+    __shared__ float maxima[kRowWarps], sums[kRowWarps];
+    constexpr int kAhead = N <= 4 ? 8 : N <= 8 ? 4 : 2;
+    pdl_enter();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint64_t item = SPLIT ? blockIdx.x : (uint64_t)blockIdx.x * kRowWarps + warp;
+    if (item >= a.queries * a.head_count) return;
+    const uint64_t row = item / a.head_count, head = item % a.head_count;
+    const SeqRow s = seq_load(a.table, seq_of_query(a.table, (uint32_t)row));
+    if constexpr (!SPLIT) {
+        attention_row<T, R, N, kAhead>(a, kr, vr, s, row, head, lane, q_shared[warp]);
+    } else {
+        float o[N], m, l;
+        attention_keys<T, R, N, kAhead>(a, kr, vr, s, row, head, lane, q_shared[warp], 32 * warp, 32 * kRowWarps, o, m, l);
+#pragma unroll
+        for (int i = 0; i < N; i++) means[warp][lane + 32 * i] = o[i];
+        if (lane == 0) {
+            maxima[warp] = m;
+            sums[warp] = l;
+        }
+        __syncthreads();
+        // the warps' means, each by its share of the weights
+        float most = __int_as_float(0xff800000), total = 0.0f, share[kRowWarps];
+#pragma unroll
+        for (int w = 0; w < kRowWarps; w++) most = fmaxf(most, maxima[w]);
+#pragma unroll
+        for (int w = 0; w < kRowWarps; w++) {
+            share[w] = sums[w] == 0.0f ? 0.0f : sums[w] * expf(maxima[w] - most);
+            total += share[w];
+        }
+        T* out = (T*)a.out + (row * a.head_count + head) * a.value_dim;
+        for (int i = threadIdx.x; i < (int)a.value_dim; i += kRowThreads) {
+            float x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kRowWarps; w++) x = fmaf(total != 0.0f ? share[w] / total : 0.0f, means[w][i], x);
+            out[i] = from_f32<T>(x);
+        }
+    }
+}
 
 template <typename T, typename R>
-__global__ void __launch_bounds__(kRowThreads) attention_packed_row_kernel(const k::PackedAttentionArgs a, R kr, R vr) {
-    pdl_enter();
-    const uint64_t warp = (uint64_t)blockIdx.x * (kRowThreads / 32) + threadIdx.x / 32;
-    if (warp >= a.queries * a.head_count) return;
-    const uint64_t row = warp / a.head_count, head = warp % a.head_count;
-    const SeqRow s = seq_load(a.table, seq_of_query(a.table, (uint32_t)row));
-    attention_row<T, R, (int)(k::kPackedMaxDim / 32)>(a, kr, vr, s, row, head, threadIdx.x % 32);
+void enqueue_rows(Device* d, const k::PackedAttentionArgs& a, unsigned blocks, bool split, const R& kr, const R& vr) {
+    auto go = [&](auto n) {
+        constexpr int N = decltype(n)::value;
+        if (split) enqueue(d, attention_packed_row_kernel<T, R, N, true>, blocks, kRowThreads, 0, a, kr, vr);
+        else enqueue(d, attention_packed_row_kernel<T, R, N, false>, blocks, kRowThreads, 0, a, kr, vr);
+    };
+    if (a.value_dim <= 128) go(std::integral_constant<int, 4>{});
+    else if (a.value_dim <= 256) go(std::integral_constant<int, 8>{});
+    else go(std::integral_constant<int, (int)(k::kPackedMaxDim / 32)>{});
 }
 
 mg_status attention_packed_rows(Device* d, const k::PackedAttentionArgs& a) {
-    const uint64_t blocks = (a.queries * a.head_count + kRowThreads / 32 - 1) / (kRowThreads / 32);
+    // A block for each while that leaves the SMs with fewer warps than they hold.
+    const uint64_t items = a.queries * a.head_count;
+    const bool split = items < (uint64_t)d->sm_count * 16;
+    const uint64_t blocks = split ? items : (items + kRowWarps - 1) / kRowWarps;
     if (blocks > 0x7fffffffull) return fail(MG_SHAPE_UNSUPPORTED, "attention launch size overflows");
     return by_float(a.dtype, [&](auto t) {
         using T = decltype(t);
         const uint64_t kw = a.kv_head_count * a.head_dim, vw = a.kv_head_count * a.value_dim;
         if (a.kv_dtype == MG_Q4) {
-            const Q4Rows kr{(const uint8_t*)a.k, kw / kQ4Block}, vr{(const uint8_t*)a.v, vw / kQ4Block};
-            enqueue(d, attention_packed_row_kernel<T, Q4Rows>, (unsigned)blocks, kRowThreads, 0, a, kr, vr);
+            enqueue_rows<T>(d, a, (unsigned)blocks, split, Q4Rows{(const uint8_t*)a.k, kw / kQ4Block}, Q4Rows{(const uint8_t*)a.v, vw / kQ4Block});
         } else {
-            const PlainRows<T> kr{(const T*)a.k, kw}, vr{(const T*)a.v, vw};
-            enqueue(d, attention_packed_row_kernel<T, PlainRows<T>>, (unsigned)blocks, kRowThreads, 0, a, kr, vr);
+            const bool vec = reinterpret_cast<uintptr_t>(a.k) % 16 == 0 && a.head_dim % 8 == 0;
+            enqueue_rows<T>(d, a, (unsigned)blocks, split, PlainRows<T>{(const T*)a.k, kw, vec}, PlainRows<T>{(const T*)a.v, vw, false});
         }
         return launched(d, "packed attention launch");
     });

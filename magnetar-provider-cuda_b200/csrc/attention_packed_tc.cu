@@ -230,13 +230,16 @@ __device__ __forceinline__ void commit(uint32_t lead, uint32_t bar) {
 
 template <typename T, int D>
 __device__ __noinline__ void recompute_rows(const Params& p, const SeqRow& s, uint32_t tok0, uint32_t head0) {
+    extern __shared__ uint8_t smem_raw[];
+    float* q_shared = reinterpret_cast<float*>(smem_raw + (-smem_u32(smem_raw) & 15u));  // (all copies and MMAs are done)
     const int lane = threadIdx.x % 32;
     const uint64_t w = p.a.kv_head_count * D;
-    const PlainRows<T> kr{(const T*)p.a.k, w}, vr{(const T*)p.a.v, w};
+    const PlainRows<T> kr{(const T*)p.a.k, w, true}, vr{(const T*)p.a.v, w, true};
     for (uint32_t r = threadIdx.x / 32 - 4; r < 2 * kRows; r += 8) {  // (by warps 4-11)
         const uint32_t tok = tok0 + (r >> p.pack_log2);
         if (tok >= s.q_count) break;
-        attention_row<T, PlainRows<T>, D / 32>(p.a, kr, vr, s, s.q_start + tok, head0 + (r & (p.pack - 1)), lane);
+        attention_row<T, PlainRows<T>, D / 32, 1>(p.a, kr, vr, s, s.q_start + tok, head0 + (r & (p.pack - 1)), lane,
+                                               q_shared + (threadIdx.x / 32 - 4) * D);
     }
 }
 
