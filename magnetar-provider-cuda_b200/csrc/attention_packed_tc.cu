@@ -24,6 +24,8 @@
 // are zeroed in shared memory, and if a remaining one is not finite the CTA's rows are computed again
 // one by one at the end.
 //
+// Few rows over many keys: the keys are split over CTAs, whose parts a second kernel joins.
+//
 // Causal, heads of 128: ten prompts of 1 to 8192 tokens, 32 heads over 8, bfloat16, 724 us, 1.04 PFLOP/s, the
 // tensor pipe busy for 58 % (the chain scores, softmax, product of two tiles sets the pace); 4 x 2048 tokens, 32
 // heads, f32, 552 us with the split, 249 TFLOP/s, three times that on the tensor cores.
@@ -47,6 +49,7 @@ constexpr int kThreads = 384;   // 12 warps
 // Registers of a thread of warps 0-3 and of warps 4-11; their sum over the block must not pass what it
 // is launched with (checked before the first launch).
 constexpr int kFewRegs = 80, kManyRegs = 200;
+constexpr uint64_t kPartKeys = 512;  // keys that a CTA of split keys has at the least
 
 template <typename T, int D>
 struct Shape {
@@ -75,6 +78,13 @@ struct Params {
     uint32_t tokens;            // of a CTA: 256 / pack
     float scale2;               // scores to log2 units
     int* error;
+    // Keys split over several CTAs: the parts, and for CTA c (of part c % parts) and its row r the mean of the
+    // part's values at means + (c * live + r) * D, the reference and the sum at stats[c * live + r], and whether
+    // the CTA met a value that asks for its rows to be computed again.
+    uint32_t parts, live;
+    float* means;
+    float2* stats;
+    uint32_t* again;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -228,6 +238,15 @@ __device__ __forceinline__ void commit(uint32_t lead, uint32_t bar) {
         : "memory");
 }
 
+// The sequence and the tokens of work item `item` (by all lanes of a warp).  Sequences with the most keys
+// first, and a sequence's last (heaviest) tokens first: CTAs start in grid order, so light ones fill the last wave.
+__device__ __forceinline__ void item_place(const Params& p, uint32_t item, uint32_t& seq, uint32_t& place) {
+    auto tiles = [&](uint32_t n) { return (n + p.tokens - 1) / p.tokens; };
+    const bool found = find_item(p.a.table, item, tiles, seq, place);
+    place = found ? tiles(__ldg(&p.a.table.ordered[seq].q_count)) - 1 - place : 0;
+    seq = found ? seq : 0xffffffffu;
+}
+
 template <typename T, int D>
 __device__ __noinline__ void recompute_rows(const Params& p, const SeqRow& s, uint32_t tok0, uint32_t head0) {
     extern __shared__ uint8_t smem_raw[];
@@ -243,7 +262,9 @@ __device__ __noinline__ void recompute_rows(const Params& p, const SeqRow& s, ui
     }
 }
 
-template <typename T, int D>
+// SPLIT: the CTA takes one of p.parts equal parts of its rows' tiles of keys, and leaves the part's means and
+// statistics to merge_parts_kernel.
+template <typename T, int D, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_packed_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                                const __grid_constant__ CUtensorMap map_klo, const __grid_constant__ CUtensorMap map_v,
@@ -290,15 +311,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_relinquish();
     }
     if (warp == 0) {
-        // Sequences with the most keys first, and a sequence's last (heaviest) tokens first: CTAs start in
-        // grid order, so light ones fill the last wave.  (The table was written by copies, which a
-        // launch never overtakes.)
+        // (the table was written by copies, which a launch never overtakes)
         uint32_t seq, place;
-        auto tiles = [&](uint32_t n) { return (n + p.tokens - 1) / p.tokens; };
-        const bool found = find_item(p.a.table, blockIdx.x / p.groups, tiles, seq, place);
+        item_place(p, (SPLIT ? blockIdx.x / p.parts : blockIdx.x) / p.groups, seq, place);
         if (lane == 0) {
-            s_seq = found ? seq : 0xffffffffu;
-            s_place = found ? tiles(__ldg(&p.a.table.ordered[seq].q_count)) - 1 - place : 0;
+            s_seq = seq;
+            s_place = place;
         }
     }
     pdl_enter();  // after the TMEM allocation, as every tensor-memory kernel here does
@@ -308,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = tmem_slot;
     const bool any = s_seq != 0xffffffffu;
     const SeqRow seq = any ? seq_load(p.a.table, p.a.table.ordered, s_seq) : SeqRow{0, 0, 0, 0};
-    const uint32_t tok0 = s_place * p.tokens, head0 = (blockIdx.x % p.groups) * p.pack;
+    const uint32_t tok0 = s_place * p.tokens, head0 = ((SPLIT ? blockIdx.x / p.parts : blockIdx.x) % p.groups) * p.pack;
     const int kvh = (int)(head0 / (uint32_t)(p.a.head_count / p.a.kv_head_count));
     const int m_keys = (int)seq.k_count, shift = m_keys - (int)seq.q_count;  // token i stands at shift + i
     const int window = p.a.window >= 0 && p.a.window < 0x7fffffff ? (int)p.a.window : -1;
@@ -320,13 +338,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     // Keys [kv0, ...) the CTA reads, and the tiles of them each query tile reads.
     const int live_tokens = min((int)p.tokens, (int)seq.q_count - (int)tok0);
-    const int kv0 = window > 0 ? max(0, shift + (int)tok0 - window + 1) : 0;
-    int n_t[2], hi_cta = 0;
+    int kv0 = window > 0 ? max(0, shift + (int)tok0 - window + 1) : 0;
+    int n_t[2], hi_cta = 0, kv_end = 0x7fffffff;
+    if constexpr (SPLIT) {
+        const int hi = p.a.causal ? min(m_keys, shift + (int)tok0 + live_tokens) : m_keys;
+        const int tiles = hi > kv0 ? (hi - kv0 + KV - 1) / KV : 0, part = (int)(blockIdx.x % p.parts);
+        const int each = (tiles + (int)p.parts - 1) / (int)p.parts;
+        kv_end = kv0 + min(tiles, (part + 1) * each) * KV;
+        kv0 += min(tiles, part * each) * KV;
+    }
 #pragma unroll
     for (int t = 0; t < 2; t++) {
         const int first = t * (int)p.tokens / 2;  // (a tile holds whole tokens: pack <= 128)
         const int last = min(live_tokens, first + (int)p.tokens / 2) - 1;
-        const int hi = last < first ? 0 : p.a.causal ? min(m_keys, shift + (int)tok0 + last + 1) : m_keys;
+        const int hi = last < first ? 0 : min(kv_end, p.a.causal ? min(m_keys, shift + (int)tok0 + last + 1) : m_keys);
         n_t[t] = hi > kv0 ? (hi - kv0 + KV - 1) / KV : 0;
         hi_cta = max(hi_cta, hi);
     }
@@ -674,11 +699,35 @@ __global__ void __launch_bounds__(kThreads, 1)
             have = !failed;
         }
         if (failed) atomicExch(p.error, 1);
+        if constexpr (SPLIT) {
+            const uint32_t row = (uint32_t)(t * kRows + r);
+            if (live) {
+                const uint64_t at = (uint64_t)blockIdx.x * p.live + row;
+                p.stats[at] = make_float2(have ? m : kNegInf, have ? l : 0.0f);
+            }
+            if (have) tc_fence_after();
+            const float inv = !have || m == kNegInf ? 0.0f : 1.0f / l;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                float o[32];
+                if (have) {
+                    tmem_ld32(tO + (uint32_t)c, o);  // (by the whole warp)
+                    tc_wait_ld();
+                }
+                if (live) {
+                    float4* dst = reinterpret_cast<float4*>(p.means + ((uint64_t)blockIdx.x * p.live + row) * D + c);
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        dst[e] = have ? make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv)
+                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
+            }
+        }
         T* out = (T*)p.a.out;
         constexpr int kChunks = D * (int)sizeof(T) / 16;  // 16-byte chunks per row
         constexpr int kRowsPerStore = 32 / kChunks;       // rows one warp store covers
         constexpr int N = 16 / (int)sizeof(T);
-        if (have) {
+        if (!SPLIT && have) {
             // Each thread writes its row into its warp's staging area -- this tile's queries, which no MMA
             // reads once the last P V has completed -- with chunk k of row i at position k ^ i; then the
             // warp stores whole rows, 16 bytes per lane.
@@ -709,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint8_t* staged = base_ptr + t * S::kQTile + qq * (32 * D * (int)sizeof(T));
         const int chunk = lane % kChunks;
 #pragma unroll 1
-        for (int i0 = lane / kChunks; i0 < 32; i0 += 4 * kRowsPerStore) {
+        for (int i0 = lane / kChunks; !SPLIT && i0 < 32; i0 += 4 * kRowsPerStore) {
             uint4 v[4];
 #pragma unroll
             for (int u = 0; u < 4; u++) {
@@ -730,7 +779,59 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
-    if (s_poison && warp >= 4) recompute_rows<T, D>(p, seq, tok0, head0);
+    if constexpr (SPLIT) {
+        if (threadIdx.x == 0) p.again[blockIdx.x] = s_poison;
+    } else {
+        if (s_poison && warp >= 4) recompute_rows<T, D>(p, seq, tok0, head0);
+    }
+}
+
+// The rows of one item from its parts: each part's mean by its share of the weights, one row per warp.
+constexpr int kMergeWarps = 4;
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * kMergeWarps) merge_parts_kernel(const Params p) {
+    __shared__ __align__(16) float q_shared[kMergeWarps][D];
+    pdl_enter();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    uint32_t id, place;
+    item_place(p, blockIdx.x / p.groups, id, place);
+    if (id == 0xffffffffu) return;
+    const SeqRow seq = seq_load(p.a.table, p.a.table.ordered, id);
+    const uint32_t tok0 = place * p.tokens, head0 = (blockIdx.x % p.groups) * p.pack;
+    const uint32_t rows = min(p.tokens, seq.q_count - tok0) * p.pack, cta0 = blockIdx.x * p.parts;
+    uint32_t again = 0;
+    for (uint32_t c = lane; c < p.parts; c += 32) again |= p.again[cta0 + c];
+    again = __any_sync(0xffffffffu, again);
+    const uint32_t r = blockIdx.y * kMergeWarps + warp;
+    if (r >= rows) return;
+    const uint64_t token = seq.q_start + tok0 + (r >> p.pack_log2), head = head0 + (r & (p.pack - 1));
+    if (again) {
+        const uint64_t w = p.a.kv_head_count * D;
+        const PlainRows<T> kr{(const T*)p.a.k, w, true}, vr{(const T*)p.a.v, w, true};
+        attention_row<T, PlainRows<T>, D / 32, 4>(p.a, kr, vr, seq, token, head, lane, q_shared[warp]);
+        return;
+    }
+    float most = __int_as_float(0xff800000), total = 0.0f, o[D / 32] = {};
+    for (uint32_t c = lane; c < p.parts; c += 32) most = fmaxf(most, p.stats[(uint64_t)(cta0 + c) * p.live + r].x);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, w));
+    // (a part of a row with a NaN or +inf score has a NaN reference, and makes the row NaN)
+    auto share = [&](uint32_t c) {
+        const float2 ml = p.stats[(uint64_t)(cta0 + c) * p.live + r];
+        return ml.y == 0.0f ? 0.0f : ml.y * exp2f(ml.x - most);
+    };
+    for (uint32_t c = lane; c < p.parts; c += 32) total += share(c);
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
+#pragma unroll 4
+    for (uint32_t c = 0; c < p.parts; c++) {
+        const float w = total == 0.0f ? 0.0f : share(c) / total;
+#pragma unroll
+        for (int i = 0; i < D / 32; i++) o[i] = fmaf(w, p.means[((uint64_t)(cta0 + c) * p.live + r) * D + lane + 32 * i], o[i]);
+    }
+    T* out = (T*)p.a.out + (token * p.a.head_count + head) * D;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) out[lane + 32 * i] = from_f32<T>(o[i]);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -771,12 +872,14 @@ mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
     static_assert(S::kSmem <= 227 * 1024 - 512, "shared memory budget");
     static bool configured[64] = {false};
     if (!configured[d->ordinal & 63]) {
-        MG_CUDA(cudaFuncSetAttribute(attention_packed_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
-                "configuring the packed attention kernel");
-        cudaFuncAttributes fa;
-        MG_CUDA(cudaFuncGetAttributes(&fa, attention_packed_tc_kernel<T, D>), "configuring the packed attention kernel");
-        if (fa.numRegs * kThreads < kFewRegs * 128 + kManyRegs * 256)
-            return fail(MG_EXECUTION_FAILED, "the packed attention kernel was built with %d registers, too few to share out", fa.numRegs);
+        for (auto kernel : {attention_packed_tc_kernel<T, D, false>, attention_packed_tc_kernel<T, D, true>}) {
+            MG_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem),
+                    "configuring the packed attention kernel");
+            cudaFuncAttributes fa;
+            MG_CUDA(cudaFuncGetAttributes(&fa, kernel), "configuring the packed attention kernel");
+            if (fa.numRegs * kThreads < kFewRegs * 128 + kManyRegs * 256)
+                return fail(MG_EXECUTION_FAILED, "the packed attention kernel was built with %d registers, too few to share out", fa.numRegs);
+        }
         configured[d->ordinal & 63] = true;
     }
     Params p;
@@ -789,6 +892,10 @@ mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
     p.tokens = 2 * kRows / p.pack;
     p.scale2 = a.scale * 1.4426950408889634f;
     p.error = d->flags + 2;
+    p.parts = p.live = 0;
+    p.means = nullptr;
+    p.stats = nullptr;
+    p.again = nullptr;
     uint64_t items = 0;
     for (const SeqRow& r : a.host->rows) items += (r.q_count + p.tokens - 1) / p.tokens;
     if (items * p.groups > 0x7fffffffull) return fail(MG_SHAPE_UNSUPPORTED, "attention launch size overflows");
@@ -824,8 +931,28 @@ mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
         maps[2] = maps[1];
         maps[4] = maps[3];
     }
-    enqueue(d, attention_packed_tc_kernel<T, D>, (unsigned)(items * p.groups), kThreads, S::kSmem, maps[0], maps[1], maps[2], maps[3],
-            maps[4], p);
+    // Fewer CTAs than half of the SMs: the keys are split, and a second kernel joins the parts.  One bfloat16 query
+    // over 32768 keys, 32 heads over 8: 516 -> 50 us; 16 queries over 4096: 67 -> 20; four of 64 to 3000 keys:
+    // 53 -> 19.  With parts of fewer than kPartKeys the join costs more than it gives (8 heads over 500 keys:
+    // 11.3 us whole, 13.3 in two parts).
+    const uint64_t ctas = items * p.groups;
+    uint64_t longest = 0;
+    for (const SeqRow& r : a.host->rows) longest = std::max<uint64_t>(longest, r.k_count + a.max_step);
+    const uint64_t parts = ctas ? std::min<uint64_t>((uint64_t)d->sm_count / ctas, longest / kPartKeys) : 0;
+    if (parts < 2) {
+        enqueue(d, attention_packed_tc_kernel<T, D, false>, (unsigned)ctas, kThreads, S::kSmem, maps[0], maps[1], maps[2], maps[3], maps[4], p);
+        return launched(d, "packed attention launch");
+    }
+    p.parts = (uint32_t)parts;
+    p.live = (uint32_t)std::min<uint64_t>(2 * kRows, a.host->max_queries * p.pack);
+    const uint64_t rows = ctas * parts * p.live;
+    MG_TRY(scratch(d, 9, rows * (D * sizeof(float) + sizeof(float2)) + ctas * parts * sizeof(uint32_t), (void**)&p.means));
+    p.stats = reinterpret_cast<float2*>(p.means + rows * D);
+    p.again = reinterpret_cast<uint32_t*>(p.stats + rows);
+    enqueue(d, attention_packed_tc_kernel<T, D, true>, (unsigned)(ctas * parts), kThreads, S::kSmem, maps[0], maps[1], maps[2], maps[3], maps[4],
+            p);
+    MG_TRY(launched(d, "packed attention launch"));
+    enqueue(d, merge_parts_kernel<T, D>, dim3((unsigned)ctas, (p.live + kMergeWarps - 1) / kMergeWarps), 32 * kMergeWarps, 0, p);
     return launched(d, "packed attention launch");
 }
 

@@ -94,6 +94,35 @@ def test_attention_packed(kernels, dtype, heads, kv, dim, queries, keys):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (8, 4, 64), (3, 3, 80), (2, 1, 200)])
+@pytest.mark.parametrize("queries,keys", [([1], [5000]), ([1, 1, 3], [2000, 1, 900]), ([40, 0, 1], [3000, 5, 64]), ([2, 300], [2, 1500])])
+def test_attention_packed_few_queries_over_many_keys(kernels, dtype, heads, kv, dim, queries, keys):
+    """Few rows, whose keys are split; a value of NaN that the last query of a sequence alone sees, and NaN behind its keys."""
+    q = randn((sum(queries), heads * dim), dtype, 11)
+    k, v = randn((sum(keys) + 1, kv * dim), dtype, 12), randn((sum(keys) + 1, kv * dim), dtype, 13)
+    k[-1], v[-1] = math.nan, math.nan
+    torch.cuda.synchronize()
+    seqs = kernels.sequences(queries, keys)
+    finite = v.clone()
+    for poison in (False, True):
+        if poison:
+            finite[sum(keys) - 1, 0] = 0
+            v[sum(keys) - 1, 0] = math.nan
+            torch.cuda.synchronize()
+        for causal, window in ((True, None), (True, 333), (False, None)):
+            got = to_torch(kernels, kernels.attention_packed(*(kernels.wrap_tensor(t) for t in (q, k, v)), seqs, heads, dim,
+                                                             kv_head_count=kv, causal=causal, window_size=window))
+            want = attention64(q, k, finite, heads, kv, queries, keys, causal=causal, window=window)
+            if poison:
+                first = sum(queries) - (1 if causal else queries[-1])
+                for h in range(heads // kv):  # the heads of that value column
+                    want[first:, h * dim] = math.nan
+            assert torch.equal(torch.isnan(got), torch.isnan(want)), (poison, causal, window)
+            fine = ~torch.isnan(want)
+            assert rel(got[fine], want[fine]) <= ATTENTION_TOL[dtype], (poison, causal, window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_attention_packed_reads_its_own_keys_only(kernels, dtype, dim):
     """Keys in slots with NaN between them, in another order than the queries; a long sequence beside short ones."""
