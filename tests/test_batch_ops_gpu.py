@@ -688,3 +688,40 @@ def test_executor_kernels(kernels, executor, mpc):
                        "ShapeUnsupported"),
                       (inv("add", ["store", "store"], "o"), "DTypeUnsupported")):
         assert executor.submit_kernel(bad).error_code == code
+
+
+def test_executor_decode_loop_over_long_plain_stores(kernels, executor, mpc):
+    """The same loop over f32 stores, with slots so long that the keys are split: the parts follow the key counts."""
+    heads, kv, dim, slot, ages = 4, 2, 64, 3000, [1500, 10, 700]
+    inv = mpc.KernelInvocation
+    total, starts = slot * 3, [0, slot, 2 * slot]
+    k, v = randn((total, kv * dim), "f32", 95), randn((total, kv * dim), "f32", 96)
+    for name, t in (("ks", k), ("vs", v)):
+        store = torch.full((total, kv * dim), math.nan, device="cuda")
+        for s, m in zip(starts, ages):
+            store[s:s + m - 1] = t[s:s + m - 1]
+        torch.cuda.synchronize()
+        executor.write_tensor(name, store.cpu().numpy())
+    executor.adopt("seqs", kernels.sequences([1, 1, 1], ages, starts))
+    offsets = [0, 1, 2, 600, 601, 1499, 1500]
+    q = randn((len(offsets), 3, heads * dim), "f32", 97)
+    torch.cuda.synchronize()
+    for name, w in (("q", heads), ("kn", kv), ("vn", kv)):
+        executor.write_zeroed_tensor(name, (3, w * dim))
+    nodes = [inv("kv-write-packed", ["ks", "kn", "seqs"], "ks"), inv("kv-write-packed", ["vs", "vn", "seqs"], "vs"),
+             inv("attention-packed", ["q", "ks", "vs", "seqs"], "out",
+                 {"head_count": heads, "head_dimension": dim, "kv_head_count": kv, "causal": True})]
+    for n in nodes:
+        executor.run(n)
+    executor.begin_step_capture(["key_count"])
+    for n in nodes:
+        executor.run(n)
+    executor.end_step_capture()
+    out, last = np.empty((3, heads * dim), np.float32), -1
+    for i, offset in enumerate(offsets):
+        for o in range(last + 1, offset + 1):  # every token is written, those at `offsets` are looked at
+            rows = [s + m - 1 + o for s, m in zip(starts, ages)]
+            executor.replay_step_io({"q": q[i].cpu().numpy(), "kn": k[rows].cpu().numpy(), "vn": v[rows].cpu().numpy()}, {"out": out}, offset=o)
+        last = offset
+        want = attention64(q[i], k, v, heads, kv, [1] * 3, [m + offset for m in ages], starts)
+        assert rel(torch.from_numpy(out).cuda(), want) <= ATTENTION_TOL["f32"], offset
