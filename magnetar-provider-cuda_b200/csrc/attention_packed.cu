@@ -99,11 +99,14 @@ namespace k {
 
 bool attention_packed_tc_eligible(const PackedAttentionArgs& a);
 mg_status attention_packed_tc(Device* d, const PackedAttentionArgs& a);
+bool attention_few_eligible(const PackedAttentionArgs& a);
+mg_status attention_few(Device* d, const PackedAttentionArgs& a);
 bool attention_q4_eligible(const PackedAttentionArgs& a);
 mg_status attention_q4(Device* d, const PackedAttentionArgs& a);
 
 mg_status attention_packed(Device* d, const PackedAttentionArgs& a) {
     if (a.queries == 0) return MG_OK;
+    if (attention_few_eligible(a)) return attention_few(d, a);
     if (attention_packed_tc_eligible(a)) return attention_packed_tc(d, a);
     if (attention_q4_eligible(a)) return attention_q4(d, a);
     return attention_packed_rows(d, a);
