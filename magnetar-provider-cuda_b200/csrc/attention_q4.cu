@@ -21,7 +21,8 @@
 //
 // The tiles (64 keys on the store's own boundaries) of all sequences and row blocks form one line per kv
 // head, each row block with a length for its own cost in front, and the line is cut into equal shares,
-// one per CTA: however ragged the batch, all CTAs have as much to do.  In
+// one per CTA: however ragged the batch, all CTAs have as much to do.  A captured step's grid is sized for the
+// keys it may grow to; of its CTAs as many have a share as the line's present length asks for.  In
 // a share a warp takes every fourth tile on its own, with its own maximum, sum and output.  The four warps'
 // results are merged in shared memory, those of a row block that was cut by the CTA that finishes last.
 //
@@ -42,6 +43,7 @@ constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 2;  // tiles of K and V a warp has in flight or in use
 constexpr int kBlockCost = 12;  // a row block's queries and merge cost as much as so many tiles
+constexpr uint64_t kLeastShare = kBlockCost + kWarps;  // units: a tile for each warp, beside a row block's cost
 constexpr int kPerSm = 3;   // CTAs of an SM: as many as shared memory holds
 
 template <int D>
@@ -157,6 +159,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
     // A sequence's units (its tiles, and what a row block costs beside them), and its row blocks.
     auto units_of = [&](const SeqRow& q) { return kBlockCost + (uint32_t)(((uint64_t)q.k_start + q.k_count + 63) / 64 - q.k_start / 64); };
     auto blocks_of = [&](const SeqRow& q) { return (q.q_count * p.group + R - 1) / R; };
+    // CTAs that have a share: all of an eager launch's grid.  No share of theirs is empty, so the last one to
+    // finish a row block is one of those that it was cut among.
+    auto shares_of = [&](uint64_t units) { return min((uint64_t)gridDim.x, max((uint64_t)1, (units + kLeastShare - 1) / kLeastShare)); };
     if (warp == 0) {
         // The line's length, and this CTA's share of it: from unit `begin` on; then the sequence it lies in.
         uint64_t units = p.units;
@@ -169,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
 #pragma unroll
             for (int w = 16; w > 0; w >>= 1) units += __shfl_xor_sync(0xffffffffu, units, w);
         }
-        const uint64_t begin = units * blockIdx.x / gridDim.x;
+        const uint64_t begin = units * blockIdx.x / shares_of(units);
         uint64_t before = 0;
         uint32_t order = 0xffffffffu;
         for (uint32_t base = 0; base < tab.count && order == 0xffffffffu; base += 32) {
@@ -201,9 +206,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
     }
     if (!tab.step) pdl_enter();
     __syncthreads();
-    const uint64_t units = s_units;
-    uint64_t pos = units * blockIdx.x / gridDim.x;
-    const uint64_t end = units * (blockIdx.x + 1) / gridDim.x;
+    const uint64_t units = s_units, grid = shares_of(units);
+    // (past the last share: past the line's end, where there is no sequence)
+    uint64_t pos = units * blockIdx.x / grid;
+    const uint64_t end = units * (blockIdx.x + 1) / grid;
     uint32_t order = s_order;
     uint64_t at = s_at;
     const int window = p.a.window > 0 && p.a.window < 0x7fffffff ? (int)p.a.window : 0;
@@ -567,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
         const bool whole_block = count == all_units;
         // This share's place among the partial results: the first of the CTA's two if it begins with the CTA's
         // own share, else the second (a share is cut at its two ends only).
-        const uint64_t begin = units * blockIdx.x / gridDim.x;
+        const uint64_t begin = units * blockIdx.x / grid;
         float* part = p.partial + (((uint64_t)blockIdx.x * p.a.kv_head_count + kvh) * 2 + (pos == begin ? 0 : 1)) * kPart;
         auto row_out = [&](int r) {
             return out + ((uint64_t)(seq.q_start + (uint32_t)((row0 + r) / (int)p.group)) * p.a.head_count + kvh * p.group +
@@ -605,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
         if (!whole_block) {
             // ---- the shares of a row block, merged by the CTA that finishes last --------------------------
             const uint64_t block_end = block_begin + all_units;
-            auto owner = [&](uint64_t unit) { return ((unit + 1) * gridDim.x - 1) / units; };  // the CTA a unit falls to
+            auto owner = [&](uint64_t unit) { return ((unit + 1) * grid - 1) / units; };  // the CTA a unit falls to
             const uint64_t cta0 = owner(block_begin), cta1 = owner(block_end - 1);
             const uint32_t shares = (uint32_t)(cta1 - cta0 + 1);
             __threadfence();
@@ -619,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
             if (s_last) {
                 __threadfence();
                 const uint64_t next = p.a.kv_head_count * 2 * (uint64_t)kPart;
-                const bool head = units * cta0 / gridDim.x == block_begin;  // the first share begins its CTA's
+                const bool head = units * cta0 / grid == block_begin;  // the first share begins its CTA's
                 const float* parts = p.partial + (cta0 * p.a.kv_head_count + kvh) * 2 * kPart;
                 auto share = [&](uint32_t i) { return parts + i * next + (i == 0 && !head ? kPart : 0); };
                 // Four columns of a row per thread, the shares taken in order, eight loads ahead; a running maximum
@@ -689,9 +695,9 @@ mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
     }
     p.units = units;
     if (a.kv_head_count > 65535) return fail(MG_SHAPE_UNSUPPORTED, "attention kv_head_count exceeds the launch grid");
-    // One wave of CTAs, each with a tile at least for each of its warps, beside a row block's cost.
+    // One wave of CTAs, each with kLeastShare at the least.
     const uint64_t wave = std::max<uint64_t>(1, (uint64_t)d->sm_count * (NT == 1 ? kPerSm : 2) / a.kv_head_count);
-    const uint64_t shares = std::max<uint64_t>(1, std::min(wave, (most + kBlockCost + kWarps - 1) / (kBlockCost + kWarps)));
+    const uint64_t shares = std::max<uint64_t>(1, std::min(wave, (most + kLeastShare - 1) / kLeastShare));
     MG_TRY(scratch(d, 9, shares * a.kv_head_count * 2 * R * (D + 2) * sizeof(float), (void**)&p.partial));
     enqueue(d, attention_q4_kernel<T, D, NT>, dim3((unsigned)shares, (unsigned)a.kv_head_count), kThreads, S::kSmem, p);
     return launched(d, "4-bit attention launch");
