@@ -25,6 +25,9 @@ constexpr int kCandidates = 512;
 static_assert(kGroups >= MG_LOGPROBS_MAX_TOP, "as many groups as top columns");
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMove = 16.0f;  // the reference moves when a value passes it by more than 2^16
+// Where the row's maximum is at least kNear above the floor it does not matter by how far logits were raised to it
+// (2^-kNear is zero in an f32 of normal range).  Other rows take a second pass.
+constexpr float kNear = 160.0f;
 
 struct LogprobsK {
     const void* logits;
@@ -34,7 +37,7 @@ struct LogprobsK {
     uint32_t vocab, top;
     float inv_temperature;
     float scale;  // logits to log2 units
-    float floor;  // logits below it are as good as excluded, and counted as it: floor * scale stays finite
+    float floor;  // logits below it are counted as it: floor * scale stays finite
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -292,8 +295,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         l += __shfl_xor_sync(0xffffffffu, l, o);
         t += __shfl_xor_sync(0xffffffffu, t, o);
     }
-    if (m < to && m > __int_as_float(0xff800000)) {
-        // No logit above the floor: the sums once more, about the largest itself.
+    if ((m - W::value(floor, 0)) * p.scale < kNear && m > __int_as_float(0xff800000)) {
+        // The sums once more, about the largest itself.
         l = t = 0.0f;
         x.for_values([&](float v, uint32_t) {
             const float d = fmaxf((v - m) * p.scale, -1e38f), w = ex2(d);

@@ -56,3 +56,61 @@ def test_captured_decode_of_young_sequences_in_long_slots(kernels, executor, mpc
         a, b = randn((rows, inner), "f32", 204), randn((inner, columns), "f32", 205)
         got = to_torch(kernels, kernels.matmul(kernels.wrap_tensor(a), kernels.wrap_tensor(b)))
         assert rel(got, a.double() @ b.double()) <= 1e-5
+
+
+# ---------------------------------------------------------------------------- log probabilities
+def check_logprobs(kernels, x, tokens, top, temperature):
+    """Against 64 bits, each value by itself.  A difference of logits over the temperature carries three roundings of
+    f32 (2^-22 of its size, below 1e-6), the log-sum some 1e-6: 1e-5 + 1e-6 |value|.  The entropy and the top
+    columns, columns included, apart from the chosen token.  Log probabilities are not positive, entropies not negative."""
+    got = to_torch(kernels, kernels.token_logprobs(kernels.wrap_tensor(x), kernels.wrap_tensor(tokens), top=top, temperature=temperature)).double()
+    z = x.double() / temperature
+    logp = torch.log_softmax(z, 1)
+    entropy = -torch.where(logp == -math.inf, 0.0, logp.exp() * logp).sum(1)
+    order = torch.sort(x.float(), dim=1, descending=True, stable=True).indices[:, :top]
+    want = torch.cat([logp.gather(1, tokens.long()[:, None]), entropy[:, None], logp.gather(1, order)], 1)
+    assert torch.equal(got[:, 2 + top:], order.double())
+    a = got[:, :2 + top]
+    assert torch.equal(torch.isnan(a), torch.isnan(want))
+    low = want < -3e38  # beyond f32
+    assert (a[low] < -3e38).all()
+    fine = torch.isfinite(want) & ~low
+    assert torch.equal(torch.isfinite(a) & ~low, fine)
+    worst = ((a - want).abs() - 1e-5 - 1e-6 * want.abs())[fine].max()
+    assert worst <= 0, worst
+    assert (a[:, 0][fine[:, 0]] <= 0).all() and (a[:, 1][fine[:, 1]] >= 0).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(6, 32000), (200, 32000), (6, 131072), (200, 1001)])
+@pytest.mark.parametrize("case", ["mask 5000", "low 100", "even", "near", "at", "steep"])
+def test_token_logprobs_at_the_low_end_of_f16(kernels, case, rows, vocab):
+    """Logits down to the type's lowest value count for what they are, whatever the maximum and the temperature."""
+    g = torch.Generator(device="cuda").manual_seed(211)
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", generator=g).float()
+    temperature = 1.0
+    if case == "mask 5000":
+        x = torch.full((rows, vocab), -65504.0, device="cuda")
+        x[:, 7] = 0.0
+        temperature = 5000.0
+    elif case == "low 100":
+        x = torch.randn((rows, vocab), device="cuda", generator=g) * 300 - 33500
+        temperature = 100.0
+    elif case == "even":
+        x = torch.full((rows, vocab), -32800.0, device="cuda")
+        x[:, 5] = -32752.0
+    elif case == "near":
+        x = torch.full((rows, vocab), -65504.0, device="cuda")
+        x[:, vocab // 2] = -65472.0
+        x[1::2, :3] = -math.inf
+        temperature = 10.0
+    elif case == "at":
+        x = torch.full((rows, vocab), -32800.0, device="cuda")
+        x[:, 9] = -32768.0
+        temperature = 8.0
+    else:
+        x = torch.randn((rows, vocab), device="cuda", generator=g) * 4
+        x[:, ::3] = -65504.0
+        temperature = 300.0
+    x = x.half()
+    torch.cuda.synchronize()
+    check_logprobs(kernels, x, tokens, 3, temperature)
