@@ -1,7 +1,9 @@
 // Log probabilities of given tokens, with entropy and top alternatives, from a row of logits.
 //
-// One pass over the row: with a reference m, d = (x - m) log2 e / temperature, l = sum 2^d and
-// t = sum d 2^d.  Then log p(x) = (x - max) / temperature - log l and the entropy is log l - ln 2 t / l.
+// One pass over the row: with c = log2 e / temperature and a reference r near the largest c x, d = c x - r, l =
+// sum 2^d and t = sum d 2^d.  The entropy is log l - ln 2 t / l, whatever the reference, and log p(x) =
+// (x - max) / temperature - log l once l is about c max itself: c max - r, which is no more than the rounding
+// of c max, is known exactly (one fused multiply-add), and so is every d up to the rounding of its own size.
 // The row is read once from memory (the top columns look at a part of it again, in the L2): 2 or 4
 // bytes a logit against one exponential and some six other instructions.
 #include <algorithm>
@@ -25,9 +27,10 @@ constexpr int kCandidates = 512;
 static_assert(kGroups >= MG_LOGPROBS_MAX_TOP, "as many groups as top columns");
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMove = 16.0f;  // the reference moves when a value passes it by more than 2^16
-// Where the row's maximum is at least kNear above the floor it does not matter by how far logits were raised to it
-// (2^-kNear is zero in an f32 of normal range).  Other rows take a second pass.
-constexpr float kNear = 160.0f;
+// The pass holds where the row's maximum is at least kNear above the floor (2^-kNear is zero in an f32 of normal
+// range, so it does not matter by how far logits were raised to it) and at most kFar (c x then rounds by no
+// more than 4, so 2^d stays in range).  Other rows -- maxima or temperatures far from the usual -- take a second pass.
+constexpr float kNear = 160.0f, kFar = 0x1p27f;
 
 struct LogprobsK {
     const void* logits;
@@ -36,8 +39,8 @@ struct LogprobsK {
     uint64_t rows;
     uint32_t vocab, top;
     float inv_temperature;
-    float scale;  // logits to log2 units
-    float floor;  // logits below it are counted as it: floor * scale stays finite
+    float scale;  // c: logits to log2 units
+    float floor;  // logits below it (excluded ones among them) are counted as it, see kNear and kFar
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -156,13 +159,14 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
 
     // ---- the row's sums -----------------------------------------------------------------------------
     const uint32_t floor = W::of(p.floor);
-    float ref = W::value(floor, 0);
+    const float low = W::value(floor, 0);
+    float ref = low * p.scale;  // in log2 units
     uint64_t l2 = f2(0.0f, 0.0f), t2 = f2(0.0f, 0.0f);
     uint32_t most = W::kExcluded;  // of the logits as they are, NaN staying NaN
     const uint64_t scale2 = f2(p.scale, p.scale);
     // l and t moved to another reference; a part of no weight adds nothing, however far away
     auto moved = [&](float to, float& l, float& t) {
-        const float d = (ref - to) * p.scale, w = ex2(d);
+        const float d = ref - to, w = ex2(d);
         t = w > 0.0f ? w * fmaf(l, d, t) : 0.0f;
         l *= w;
     };
@@ -173,8 +177,8 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         for (int i = 4; i < kWords; i++) top[i % 4] = W::larger(top[i % 4], w[i]);
         const uint32_t all = W::larger(W::larger(top[0], top[1]), W::larger(top[2], top[3]));
         most = W::larger(most, all);
-        const float to = W::largest(all);
-        if ((to - ref) * p.scale > kMove) {
+        if (fmaf(W::largest(all), p.scale, -ref) > kMove) {
+            const float to = W::largest(all) * p.scale;
             float2 l = f2split(l2), t = f2split(t2);
             moved(to, l.x, t.x);
             moved(to, l.y, t.y);
@@ -182,8 +186,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
             t2 = f2(t.x, t.y);
             ref = to;
         }
-        const float r = -ref * p.scale;
-        const uint64_t ref2 = f2(r, r);
+        const uint64_t ref2 = f2(-ref, -ref);
 #pragma unroll
         for (int b = 0; b < kBatch; b++) {
             if (b >= n) break;
@@ -233,18 +236,15 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
     float mine = max_nan(W::largest(most), lone);
     float2 ll = f2split(l2), tt = f2split(t2);
     float l = ll.x + ll.y, t = tt.x + tt.y;
-    // excluded logits that were counted at the floor, while the reference lay there
-    {
-        const float low = W::value(floor, 0), v = max_nan(lone, low);
-        if (v > ref) {
-            moved(v, l, t);
-            ref = v;
+    if (has_single) {
+        const float v = max_nan(lone, low), to = v * p.scale;
+        if (to > ref) {
+            moved(to, l, t);
+            ref = to;
         }
-        if (has_single) {
-            const float d = (v - ref) * p.scale, w = ex2(d);
-            l += w;
-            t = fmaf(w, d, t);
-        }
+        const float d = fmaf(v, p.scale, -ref), w = ex2(d);
+        l += w;
+        t = fmaf(w, d, t);
     }
     // ---- the block's ----------------------------------------------------------------------------------
     float m = mine;
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
     m = warp_max[lane % kWarps];
 #pragma unroll
     for (int o = 1; o < kWarps; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float to = max_nan(m, W::value(floor, 0));
+    const float to = max_nan(m, low) * p.scale;
     moved(to, l, t);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -295,8 +295,11 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
         l += __shfl_xor_sync(0xffffffffu, l, o);
         t += __shfl_xor_sync(0xffffffffu, t, o);
     }
-    if ((m - W::value(floor, 0)) * p.scale < kNear && m > __int_as_float(0xff800000)) {
+    float lost = fmaf(m, p.scale, -to);  // by the rounding of c m
+    const float over = (m - low) * p.scale;
+    if (!(over >= kNear && over <= kFar) && m > __int_as_float(0xff800000)) {
         // The sums once more, about the largest itself.
+        lost = 0.0f;
         l = t = 0.0f;
         x.for_values([&](float v, uint32_t) {
             const float d = fmaxf((v - m) * p.scale, -1e38f), w = ex2(d);
@@ -323,13 +326,18 @@ __global__ void __launch_bounds__(kThreads, kPerSm / kThreads) logprobs_kernel(c
     // A log probability is (x - m) / temperature - log l, which keeps its digits where m is large; NaN where
     // there is no distribution (no finite logit, an infinite one, a NaN).
     const float nan = __int_as_float(0x7fc00000);
-    const float log_l = m > __int_as_float(0xff800000) && m < __int_as_float(0x7f800000) ? logf(l) : nan;
-    auto logprob = [&](float v) { return (v - m) * p.inv_temperature - log_l; };
+    const float log_l = m > __int_as_float(0xff800000) && m < __int_as_float(0x7f800000) ? fmaf(-kLn2, lost, logf(l)) : nan;
+    // (no probability is above one, and no entropy below zero, by a rounding either; NaN stays)
+    auto logprob = [&](float v) {
+        const float x = (v - m) * p.inv_temperature - log_l;
+        return x > 0.0f ? 0.0f : x;
+    };
     if (threadIdx.x == 0) {
         const float id = p.tokens ? p.tokens[row] : -1.0f;
         const bool is_column = id >= 0.0f && id < (float)p.vocab && id == floorf(id);
         out[0] = is_column ? logprob(to_f32(x.x[(uint32_t)id])) : nan;
-        out[1] = log_l - t * kLn2 / l;  // log sum e^z - sum p z
+        const float entropy = log_l - kLn2 * (t / l - lost);  // log sum e^z - sum p z
+        out[1] = entropy < 0.0f ? 0.0f : entropy;
     }
     if (!p.top) return;
     if (log_l != log_l) {
@@ -449,9 +457,10 @@ mg_status token_logprobs(Device* d, const LogprobsArgs& a) {
     if (a.rows > 0x7fffffffull) return fail(MG_SHAPE_UNSUPPORTED, "token log probabilities of too many rows");
     LogprobsK p{a.logits, a.tokens, a.out, a.rows, (uint32_t)a.vocab, a.top, 1.0f / a.temperature, 0.0f, 0.0f};
     p.scale = 1.4426950408889634f * p.inv_temperature;
-    // a power of two, so that floor * scale is exact: logits at the floor are at no distance from it
-    p.floor = -exp2f(floorf(log2f(1e38f / std::max(1.0f, p.scale))));
-    if (a.dtype == MG_F16) p.floor = std::max(p.floor, -32768.0f);
+    // Half of kFar away from zero (a power of two in logits, which every type holds), or f16's lowest value, where only
+    // -inf is below it.
+    p.floor = -exp2f(floorf(log2f(std::min(1e38f, 0.5f * kFar / p.scale))));
+    if (a.dtype == MG_F16) p.floor = std::max(p.floor, -65504.0f);
     return by_float(a.dtype, [&](auto t) {
         using T = decltype(t);
         // A block of 1024 threads where the rows leave SMs free and are long enough: 8 and 148 rows of 128 KB

@@ -114,3 +114,55 @@ def test_token_logprobs_at_the_low_end_of_f16(kernels, case, rows, vocab):
     x = x.half()
     torch.cuda.synchronize()
     check_logprobs(kernels, x, tokens, 3, temperature)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,vocab", [(5, 32000), (300, 5000), (3, 200)])
+@pytest.mark.parametrize("most,temperature", [(30.1, 0.01), (5000.7, 0.1), (5000.7, 0.01), (-5000.7, 0.01), (30.1, 1e-6), (3.0, 1e-30),
+                                              (-40000.0, 1.0), (3.0, 1e4), (1e9, 1.0), (-1e9, 0.5), (3e38, 1.0), (3e38, 1e30), (-3e38, 1e30)])
+def test_token_logprobs_of_large_logits_and_far_temperatures(kernels, dtype, rows, vocab, most, temperature):
+    """One column above the others by far, two close ones, and a spread about the maximum, where the quotient of
+    logit and temperature is far from zero: the log-sum keeps its digits."""
+    limit = float(torch.finfo(DT[dtype]).max)
+    most = max(-limit, min(limit, most))
+    x = randn((rows, vocab), "f32", 212)
+    x[0] -= x[0].abs().max() + 1
+    x[0, 77] = 0.0                      # (a probability of one at low temperatures)
+    x[1] = -abs(x[1])
+    x[1, [3, vocab - 2]] = 0.0          # two alike
+    unit = min(max(temperature, 1e-30), 1e37)
+    x = (most + x.double() * 2 * unit).clamp(-limit, limit).float().to(DT[dtype])
+    tokens = torch.randint(0, vocab, (rows,), device="cuda").float()
+    tokens[0], tokens[1] = 77, 3
+    torch.cuda.synchronize()
+    check_logprobs(kernels, x, tokens, 5, temperature)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("mask", [-1e4, -1e9, -1e10, -3.3e15, -1e30, -1.7e38])
+@pytest.mark.parametrize("rows", [4, 200])
+def test_token_logprobs_beside_large_negative_masks(kernels, dtype, mask, rows):
+    """Whole stretches of a row hold a mask's value, as large as callers choose them."""
+    vocab = 40000
+    x = randn((rows, vocab), dtype, 213, 3.0)
+    x[:, : vocab - 500] = mask
+    x[1::2] = x[1::2].flip(1)
+    tokens = torch.randint(0, vocab, (rows,), device="cuda").float()
+    tokens[0] = vocab - 3
+    torch.cuda.synchronize()
+    check_logprobs(kernels, x, tokens, 7, 1.0)
+    x[:] = mask  # and nothing else
+    torch.cuda.synchronize()
+    check_logprobs(kernels, x, tokens, 7, 1.0)
+
+
+def test_token_logprobs_by_the_value(kernels):
+    """The cases of ordinary logits, each value held to its own size rather than to the largest of the tensor."""
+    for i, (dtype, rows, vocab, top, temperature) in enumerate([("f32", 8, 32000, 5, 1.0), ("bf16", 300, 999, 64, 1.0), ("f16", 5, 50001, 20, 1.3),
+                                                                ("f16", 160, 1024, 1, 1.0), ("f32", 3, 5, 5, 0.7), ("bf16", 2, 131073, 32, 1.0)]):
+        x = randn((rows, vocab), dtype, 214 + i, 3.0)
+        x[::3, : vocab // 2] = -math.inf
+        x[1::3, ::2] = torch.finfo(DT[dtype]).min
+        tokens = torch.randint(0, vocab, (rows,), device="cuda").float()
+        torch.cuda.synchronize()
+        check_logprobs(kernels, x, tokens, top, temperature)
