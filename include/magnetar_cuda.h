@@ -383,7 +383,7 @@ mg_status mg_rope_axes(mg_device* d, const mg_buffer* x, const mg_buffer* positi
 
 /* Log probabilities of given tokens, with entropy and top alternatives: logits [rows, vocab] (f32,
  * f16 or bf16), tokens [rows] f32 holding integers (NULL: none), top 0 to 64 and at most vocab,
- * temperature finite and positive.  out [rows, 2 + 2 * top] f32: the token's log probability, the
+ * temperature finite and at least FLT_MIN (1.2e-38).  out [rows, 2 + 2 * top] f32: the token's log probability, the
  * row's entropy (natural logarithms), the log probabilities of the `top` likeliest columns in
  * falling order (equal logits: the lowest column first), then those columns.  A token that is not
  * a column gives NaN (as does a NULL `tokens`), so rows without one may hold -1.  A logit of -inf

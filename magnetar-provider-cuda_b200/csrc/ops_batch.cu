@@ -5,6 +5,7 @@
 // enqueues its kernels; none of them waits for the device.  The reference serves one sequence per
 // call and has no counterpart of these entries.
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstring>
 #include <new>
@@ -477,6 +478,7 @@ mg_status mg_token_logprobs(mg_device* h, const mg_buffer* lh, const mg_buffer* 
         return fail(MG_SHAPE_UNSUPPORTED, "%u top columns exceed %d or the %llu columns", top, MG_LOGPROBS_MAX_TOP, (ull)vocab);
     if (!std::isfinite(temperature) || !(temperature > 0.0f))
         return fail(MG_SHAPE_UNSUPPORTED, "temperature %g must be finite and positive", (double)temperature);
+    if (temperature < FLT_MIN) return fail(MG_SHAPE_UNSUPPORTED, "temperature %g has no reciprocal in f32", (double)temperature);
     if (th) {
         MG_TRY(need(d, th, "tokens"));
         t = buf(th);

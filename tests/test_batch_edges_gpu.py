@@ -166,3 +166,11 @@ def test_token_logprobs_by_the_value(kernels):
         tokens = torch.randint(0, vocab, (rows,), device="cuda").float()
         torch.cuda.synchronize()
         check_logprobs(kernels, x, tokens, top, temperature)
+
+
+def test_token_logprobs_refuses_temperatures_without_a_reciprocal(kernels, mpc):
+    x = kernels.zeros((2, 8))
+    for t in (1e-39, 1e-45):
+        with pytest.raises(mpc.CudaError) as e:
+            kernels.token_logprobs(x, temperature=t)
+        assert e.value.code == "ShapeUnsupported"
