@@ -100,7 +100,9 @@ mg_status mg_device_synchronize(mg_device* device);
 /* The device's cudaStream_t (as void*). */
 void* mg_device_stream(mg_device* device);
 /* Makes the device enqueue on `stream` (a cudaStream_t of the same device) instead of
- * its own; NULL restores its own stream. */
+ * its own; NULL restores its own stream.  What the device enqueues there comes after what it has
+ * enqueued so far: its calls share workspaces and never overlap.  `stream` has to exist until
+ * another one is set or the device is closed.  MG_CAPTURE_UNSUPPORTED while a step capture records. */
 mg_status mg_device_set_stream(mg_device* device, void* stream);
 /* Upload/download counters (src/kernels.rs:546-552, 1453-1466). */
 mg_status mg_device_counters(mg_device* device, uint64_t* uploads, uint64_t* downloads);

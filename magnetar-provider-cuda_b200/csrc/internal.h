@@ -45,6 +45,7 @@ struct Device {
     int ordinal = 0;
     cudaStream_t own_stream = nullptr;
     cudaStream_t stream = nullptr;  // where work is enqueued
+    cudaEvent_t order = nullptr;    // orders one stream behind another (made at its first use)
     cudaMemPool_t pool = nullptr;
     int sm_count = 148;
     int sm_major = 10, sm_minor = 0;

@@ -335,6 +335,7 @@ void device_unref(Device* d) {
     cudaFree(d->counters);
     cudaFreeHost(d->host_flags);
     cudaMemPoolDestroy(d->pool);
+    if (d->order) cudaEventDestroy(d->order);
     cudaStreamDestroy(d->own_stream);
     delete d;
 }
@@ -487,9 +488,36 @@ mg_status mg_device_synchronize(mg_device* h) {
 
 void* mg_device_stream(mg_device* h) { return h ? (void*)dev(h)->stream : nullptr; }
 
+}  // extern "C"
+
+// Work enqueued on `later` from now on waits for what is on `first` so far.  A stream that a graph capture of the
+// caller's records takes no part: its work runs with the graph, which the caller orders.
+static mg_status order_behind(Device* d, cudaStream_t later, cudaStream_t first) {
+    for (cudaStream_t s : {later, first}) {
+        cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(s, &status) != cudaSuccess || status != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
+            return MG_OK;
+        }
+    }
+    if (!d->order) MG_CUDA(cudaEventCreateWithFlags(&d->order, cudaEventDisableTiming), "creating an event");
+    MG_CUDA(cudaEventRecord(d->order, first), "recording a stream's work");
+    MG_CUDA(cudaStreamWaitEvent(later, d->order, 0), "ordering a stream behind another");
+    return MG_OK;
+}
+
+extern "C" {
+
+// Workspaces, arrival counters and the memory pool belong to the device, whatever stream its work is on: the
+// new stream's work comes after the old one's.
 mg_status mg_device_set_stream(mg_device* h, void* stream) {
-    if (!h) return fail(MG_INVALID_ARGUMENT, "null device handle");
-    dev(h)->stream = stream ? (cudaStream_t)stream : dev(h)->own_stream;
+    MG_TRY(device_check(h));
+    Device* d = dev(h);
+    cudaStream_t next = stream ? (cudaStream_t)stream : d->own_stream;
+    if (next == d->stream) return MG_OK;
+    if (d->capturing) return fail(MG_CAPTURE_UNSUPPORTED, "the stream cannot change while a step capture records");
+    MG_TRY(order_behind(d, next, d->stream));
+    d->stream = next;
     return MG_OK;
 }
 

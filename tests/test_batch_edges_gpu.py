@@ -174,3 +174,40 @@ def test_token_logprobs_refuses_temperatures_without_a_reciprocal(kernels, mpc):
         with pytest.raises(mpc.CudaError) as e:
             kernels.token_logprobs(x, temperature=t)
         assert e.value.code == "ShapeUnsupported"
+
+
+# ---------------------------------------------------------------------------- streams
+def test_stream_changed_while_work_is_under_way(kernels, mpc, executor):
+    """Calls in turn on two streams, each with work of its own in front: they share workspaces (the split keys of f32
+    prompts, parts of keys, arrival counters), and do not overlap."""
+    heads, kv, dim = 8, 2, 128
+    busy = randn((2048, 2048), "f32", 221)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    prompts, many = [700, 300, 41], [20000]
+    calls = []
+    for i in range(8):
+        n, m = (prompts, prompts) if i % 4 < 2 else ([1], many)
+        q = randn((sum(n), heads * dim), "f32" if i % 4 < 2 else "bf16", 222 + 3 * i)
+        dtype = "f32" if i % 4 < 2 else "bf16"
+        k, v = randn((sum(m), kv * dim), dtype, 223 + 3 * i), randn((sum(m), kv * dim), dtype, 224 + 3 * i)
+        calls.append((q, k, v, kernels.sequences(n, m), torch.empty_like(q), attention64(q, k, v, heads, kv, n, m), dtype))
+    torch.cuda.synchronize()
+    try:
+        for i, (q, k, v, seqs, out, _, _) in enumerate(calls):
+            side = streams[i % 2]
+            with torch.cuda.stream(side):
+                for _ in range(3 * (i % 2)):
+                    busy @ busy
+            kernels.set_stream(side.cuda_stream)
+            kernels.attention_packed(*(kernels.wrap_tensor(t) for t in (q, k, v)), seqs, heads, dim, kv_head_count=kv, out=kernels.wrap_tensor(out))
+        executor.write_zeroed_tensor("x", (4, 64))
+        executor.begin_step_capture()
+        with pytest.raises(mpc.CudaError) as e:
+            kernels.set_stream(None)
+        assert e.value.code == "CaptureUnsupported"
+        executor.abort_step_capture()
+    finally:
+        kernels.set_stream(None)
+    torch.cuda.synchronize()
+    for *_, out, want, dtype in calls:
+        assert rel(out, want) <= ATTENTION_TOL[dtype]
