@@ -104,6 +104,10 @@ void* mg_device_stream(mg_device* device);
  * enqueued so far: its calls share workspaces and never overlap.  `stream` has to exist until
  * another one is set or the device is closed.  MG_CAPTURE_UNSUPPORTED while a step capture records. */
 mg_status mg_device_set_stream(mg_device* device, void* stream);
+/* What the device enqueues from now on waits for what is on `stream` so far (NULL: the default
+ * stream): for memory that another stream's work fills, called before the device's first call
+ * that reads it.  Nothing while either stream is being captured. */
+mg_status mg_device_wait_stream(mg_device* device, void* stream);
 /* Upload/download counters (src/kernels.rs:546-552, 1453-1466). */
 mg_status mg_device_counters(mg_device* device, uint64_t* uploads, uint64_t* downloads);
 /* Number of kernels this library has launched on the device since it was opened. */

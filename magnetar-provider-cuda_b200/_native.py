@@ -117,6 +117,7 @@ SIGNATURES = {
     "mg_device_synchronize": [_P],
     "mg_device_stream": [_P],
     "mg_device_set_stream": [_P, _P],
+    "mg_device_wait_stream": [_P, _P],
     "mg_device_counters": [_P, _U64P, _U64P],
     "mg_device_launch_count": [_P],
     "mg_buffer_create": [_P, _I, _I, _U64P, _PP],

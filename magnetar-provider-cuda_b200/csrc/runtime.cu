@@ -521,6 +521,15 @@ mg_status mg_device_set_stream(mg_device* h, void* stream) {
     return MG_OK;
 }
 
+mg_status mg_device_wait_stream(mg_device* h, void* stream) {
+    MG_TRY(device_check(h));
+    Device* d = dev(h);
+    // (the default stream has two names)
+    auto same = [](cudaStream_t a, cudaStream_t b) { return a == b || ((!a || a == cudaStreamLegacy) && (!b || b == cudaStreamLegacy)); };
+    if (same((cudaStream_t)stream, d->stream)) return MG_OK;
+    return order_behind(d, d->stream, (cudaStream_t)stream);
+}
+
 mg_status mg_device_counters(mg_device* h, uint64_t* uploads, uint64_t* downloads) {
     if (!h) return fail(MG_INVALID_ARGUMENT, "null device handle");
     if (uploads) *uploads = dev(h)->uploads.load();

@@ -234,11 +234,15 @@ class CudaKernels:
         return DeviceBuffer(out.value, self, owner)
 
     def wrap_tensor(self, t) -> DeviceBuffer:
-        """A view of a contiguous CUDA torch tensor (f32, f16 or bf16) without a copy."""
+        """A view of a contiguous CUDA torch tensor (f32, f16 or bf16) of this device without a copy.  The
+        device's next calls wait for what torch's current stream holds at this point (such as the work that
+        fills ``t``); for what is put there later, and for torch to read results, the two are ordered by the caller
+        (``synchronize``, or one stream for both: ``set_stream``)."""
         import torch
-        if not t.is_cuda or not t.is_contiguous():
-            raise CudaError(3, "only contiguous CUDA tensors can be wrapped")
+        if not t.is_cuda or not t.is_contiguous() or t.device.index != self.ordinal:
+            raise CudaError(3, f"only contiguous tensors of cuda:{self.ordinal} can be wrapped")
         dt = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"}[t.dtype]
+        check(N.lib().mg_device_wait_stream(self._h, ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)))
         return self.wrap(t.data_ptr(), tuple(t.shape), dt, owner=t)
 
     # ---- batches of packed sequences ---------------------------------------------------

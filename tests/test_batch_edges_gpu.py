@@ -211,3 +211,31 @@ def test_stream_changed_while_work_is_under_way(kernels, mpc, executor):
     torch.cuda.synchronize()
     for *_, out, want, dtype in calls:
         assert rel(out, want) <= ATTENTION_TOL[dtype]
+
+
+@pytest.mark.parametrize("side", [False, True])
+def test_wrapped_tensors_that_torch_is_still_filling(kernels, mpc, side):
+    """torch's stream and the device's own are apart: a call waits for the work that was under way on torch's
+    current stream when the tensor was wrapped."""
+    busy, x = randn((4096, 4096), "f32", 231), randn((300, 512), "f32", 232)
+    stream = torch.cuda.Stream() if side else torch.cuda.current_stream()
+    late = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for _ in range(20):
+            busy @ busy
+        late.copy_(x)
+        buf = kernels.wrap_tensor(late)
+    got = kernels.download(kernels.add(buf, buf))
+    assert np.array_equal(got, 2 * x.cpu().numpy())
+    torch.cuda.synchronize()
+    with pytest.raises(mpc.CudaError):
+        kernels.wrap_tensor(x.cpu())
+    kernels.set_stream(1)  # torch's default stream by its other name
+    try:
+        with torch.cuda.stream(torch.cuda.default_stream()):
+            y = x + 1
+            got = kernels.download(kernels.add(kernels.wrap_tensor(y), kernels.wrap_tensor(y)))
+        assert np.array_equal(got, (2 * (x + 1)).cpu().numpy())
+    finally:
+        kernels.set_stream(None)
