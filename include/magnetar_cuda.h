@@ -348,7 +348,8 @@ mg_status mg_sequences_write(mg_buffer* sequences, uint64_t count, const uint64_
 mg_status mg_kv_store_q4(mg_device* d, uint64_t rows, uint64_t head_count, uint64_t head_dimension, mg_buffer** out);
 /* mg_kv_write accepts an MG_Q4 store, with f32, f16 or bf16 rows. */
 /* Packed kv-write: the packed rows [total queries, width] become the last query_counts[i] of each
- * sequence's key rows in `store` (f32, f16 or bf16 as the rows, or MG_Q4 with any of them). */
+ * sequence's key rows in `store` (f32, f16 or bf16 as the rows, or MG_Q4 with any of them).  Sequences
+ * whose rows would meet there are MG_SHAPE_UNSUPPORTED (reads may share rows). */
 mg_status mg_kv_write_packed(mg_device* d, mg_buffer* store, const mg_buffer* rows, const mg_buffer* sequences);
 /* The values those rows stand for: [total queries, width] f32, read back from an MG_Q4 store. */
 mg_status mg_kv_read_packed(mg_device* d, const mg_buffer* store, const mg_buffer* sequences, mg_buffer** out);

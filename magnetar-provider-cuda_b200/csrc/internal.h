@@ -137,8 +137,10 @@ struct SequenceTable {
     uint64_t key_end = 0;      // one past the last key row any sequence reads
     uint64_t max_queries = 0;  // of one sequence
     bool writable = true;      // no sequence has fewer keys than queries
-    // Keys every sequence may gain before one of them runs into the rows of another.
-    uint64_t slack = UINT64_MAX;
+    bool shared_rows = false;  // the last `queries` key rows of two sequences meet: written, they would be two things
+    // Keys every sequence may gain before one with queries runs into the rows of another; `write_slack` also where the
+    // next row is already another one's in the middle (rows that several sequences read may grow, not be written).
+    uint64_t slack = UINT64_MAX, write_slack = UINT64_MAX;
 };
 
 struct Buffer {

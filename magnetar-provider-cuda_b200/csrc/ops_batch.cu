@@ -71,17 +71,29 @@ mg_status make_table(uint64_t count, const uint64_t* query_counts, const uint64_
         t->max_queries = std::max(t->max_queries, n);
         if (m < n) t->writable = false;
     }
-    // What each sequence may grow by: up to the first row another one starts at, at or past its end.
-    std::vector<uint32_t> starts;
-    starts.reserve(count);
-    for (const SeqRow& r : t->rows)
-        if (r.k_count) starts.push_back(r.k_start);
-    std::sort(starts.begin(), starts.end());
+    // What each sequence with queries may grow by: up to the first row another one starts at, at or past its end
+    // (a sequence without queries is neither read nor written).
+    std::vector<std::pair<uint32_t, uint32_t>> spans, written;  // [start, end) of all keys, by their starts; of the written rows
+    spans.reserve(count);
+    written.reserve(count);
     for (const SeqRow& r : t->rows) {
         const uint32_t end = r.k_start + r.k_count;
-        auto it = std::lower_bound(starts.begin(), starts.end(), end);
-        if (it != starts.end()) t->slack = std::min<uint64_t>(t->slack, *it - end);
+        if (r.k_count) spans.emplace_back(r.k_start, end);
+        if (r.q_count && r.q_count <= r.k_count) written.emplace_back(end - r.q_count, end);
     }
+    std::sort(spans.begin(), spans.end());
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); i++) t->shared_rows = t->shared_rows || written[i].first < written[i - 1].second;
+    std::vector<uint32_t> farthest(spans.size());  // end of the spans up to each
+    for (size_t i = 0; i < spans.size(); i++) farthest[i] = std::max(spans[i].second, i ? farthest[i - 1] : 0u);
+    for (const SeqRow& r : t->rows) {
+        if (!r.q_count) continue;
+        const uint32_t end = r.k_start + r.k_count;
+        const size_t i = std::lower_bound(spans.begin(), spans.end(), std::make_pair(end, 0u)) - spans.begin();
+        if (i < spans.size()) t->slack = std::min<uint64_t>(t->slack, spans[i].first - end);
+        if (i && farthest[i - 1] > end) t->write_slack = 0;
+    }
+    t->write_slack = std::min(t->write_slack, t->slack);
     return MG_OK;
 }
 
@@ -168,10 +180,11 @@ mg_status kv_write_packed_plan(mg_device* h, mg_buffer* sh, const mg_buffer* rh,
     if (count != t->queries)
         return fail(MG_SHAPE_UNSUPPORTED, "the sequences have %llu rows, got %llu", (ull)t->queries, (ull)count);
     if (!t->writable) return fail(MG_SHAPE_UNSUPPORTED, "a sequence has fewer keys than rows to write");
+    if (t->shared_rows) return fail(MG_SHAPE_UNSUPPORTED, "two sequences would write the same rows of the store");
     if (t->key_end > capacity)
         return fail(MG_SHAPE_UNSUPPORTED, "the sequences' keys end at row %llu of the store's %llu", (ull)t->key_end,
                     (ull)capacity);
-    *headroom = std::min(t->slack, capacity - t->key_end);
+    *headroom = std::min(t->write_slack, capacity - t->key_end);
     a->rows = rows->ptr;
     a->dtype = rows->dtype;
     a->store = store->ptr;

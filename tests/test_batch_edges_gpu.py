@@ -239,3 +239,44 @@ def test_wrapped_tensors_that_torch_is_still_filling(kernels, mpc, side):
         assert np.array_equal(got, (2 * (x + 1)).cpu().numpy())
     finally:
         kernels.set_stream(None)
+
+
+# ---------------------------------------------------------------------------- tables whose sequences meet
+def test_sequences_that_would_write_the_same_rows_are_refused(kernels, mpc):
+    """Two sequences may read the same rows; rows written by both would be of neither."""
+    rows = randn((4, 64), "f32", 241)
+    buf = kernels.wrap_tensor(rows)
+    for store in (kernels.kv_store_q4(100, 1, 64), kernels.zeros((100, 64))):
+        for queries, keys, starts in (([2, 2], [10, 10], [0, 0]), ([2, 2], [10, 11], [0, 0]), ([3, 1], [50, 8], [0, 40]), ([1, 3], [8, 9], [41, 40])):
+            with pytest.raises(mpc.CudaError) as e:
+                kernels.kv_write_packed(store, buf, kernels.sequences(queries, keys, starts))
+            assert e.value.code == "ShapeUnsupported"
+        for queries, keys, starts in (([2, 2], [10, 12], [0, 0]), ([4, 0], [10, 10], [0, 0]), ([1, 3], [8, 8], [43, 40]), ([0, 4, 0], [0, 4, 0], [0, 0, 0])):
+            kernels.kv_write_packed(store, buf, kernels.sequences(queries, keys, starts))
+    # attention over shared rows stays as it was
+    q, k, v = randn((4, 64), "f32", 242), randn((20, 64), "f32", 243), randn((20, 64), "f32", 244)
+    got = to_torch(kernels, kernels.attention_packed(*(kernels.wrap_tensor(t) for t in (q, k, v)), kernels.sequences([2, 2], [20, 20], [0, 0]), 1, 64))
+    assert rel(got, attention64(q, k, v, 1, 1, [2, 2], [20, 20], [0, 0])) <= ATTENTION_TOL["f32"]
+
+
+@pytest.mark.parametrize("queries,keys,starts,write,read", [
+    ([1, 1], [10, 10], [0, 40], 30, 30),           # up to the second one's first row
+    ([1, 1], [10, 12], [0, 0], 0, 88),             # the first one's next row is the second one's
+    ([1, 0], [10, 50], [0, 5], 0, 45),             # ... also where that one does not write
+    ([1, 0], [50, 10], [0, 0], 50, 50),            # a sequence that only reads a part of the rows
+    ([1, 0, 1], [10, 0, 20], [0, 10, 60], 20, 20),  # an empty place in the batch
+    ([0, 1], [10, 10], [0, 10], 80, 80),           # a finished sequence in front of the one that grows
+])
+def test_how_far_a_captured_step_may_advance(kernels, executor, mpc, queries, keys, starts, write, read):
+    inv = mpc.KernelInvocation
+    n = sum(queries)
+    executor.adopt("store", kernels.kv_store_q4(100, 1, 64))
+    executor.adopt("seqs", kernels.sequences(queries, keys, starts))
+    executor.write_tensor("x", np.ones((n, 64), np.float32))
+    for node, most in ((inv("kv-write-packed", ["store", "x", "seqs"], "store"), write),
+                       (inv("attention-packed", ["x", "store", "store", "seqs"], "out", {"head_count": 1, "head_dimension": 64, "causal": True}), read)):
+        executor.run(node)
+        executor.begin_step_capture(["key_count"])
+        executor.run(node)
+        executor.end_step_capture()
+        assert executor.step_max_offset() == min(most, 100 - max(s + k for s, k in zip(starts, keys))), node
