@@ -551,7 +551,13 @@ mg_status dispatch(mg_executor* ex, const mg_invocation* inv, mg_buffer** out) {
     if (!strcmp(name, "kv-read-packed")) {
         MG_TRY(get_input(ex, inv, 0, &a));
         MG_TRY(get_input(ex, inv, 1, &b));
-        return mg_kv_read_packed(dh, H(a), H(b), out);
+        k::KvPackedArgs kp;
+        float* values;
+        uint64_t headroom;
+        MG_TRY(kv_read_packed_plan(dh, H(a), H(b), out, &kp, &values, &headroom));
+        // an advancing key_count moves the rows on, as those of kv-write-packed
+        kp.table.step = advancing_offset(ex, "key_count", headroom);
+        return k::kv_read_packed(ex->device, kp, values);
     }
     if (!strcmp(name, "attention-packed")) {
         // inputs: q, k, v, sequences

@@ -464,6 +464,8 @@ mg_status attention_plan(mg_device* h, const mg_buffer* q, const mg_buffer* k, c
 // keys a captured step may add to every sequence.
 mg_status kv_write_packed_plan(mg_device* h, mg_buffer* store, const mg_buffer* rows, const mg_buffer* sequences,
                                k::KvPackedArgs* a, uint64_t* headroom);
+mg_status kv_read_packed_plan(mg_device* h, const mg_buffer* store, const mg_buffer* sequences, mg_buffer** out,
+                              k::KvPackedArgs* a, float** values, uint64_t* headroom);
 mg_status attention_packed_plan(mg_device* h, const mg_buffer* q, const mg_buffer* k, const mg_buffer* v,
                                 const mg_buffer* sequences, const mg_attention_params* p, mg_buffer** out,
                                 k::PackedAttentionArgs* a, uint64_t* headroom);

@@ -195,6 +195,34 @@ mg_status kv_write_packed_plan(mg_device* h, mg_buffer* sh, const mg_buffer* rh,
     return MG_OK;
 }
 
+mg_status kv_read_packed_plan(mg_device* h, const mg_buffer* sh, const mg_buffer* seqs, mg_buffer** out, k::KvPackedArgs* a,
+                              float** values, uint64_t* headroom) {
+    MG_TRY(device_check(h));
+    Device* d = dev(h);
+    MG_TRY(need(d, sh, "store"));
+    const Buffer* store = buf(sh);
+    if (store->dtype != MG_Q4) return fail(MG_DTYPE_UNSUPPORTED, "kv-read reads 4-bit stores, got %s", dtype_name(store->dtype));
+    const SequenceTable* t;
+    MG_TRY(need_table(d, seqs, &t, &a->table));
+    if (!t->writable) return fail(MG_SHAPE_UNSUPPORTED, "a sequence has fewer keys than rows to read");
+    if (t->key_end > store->shape[0])
+        return fail(MG_SHAPE_UNSUPPORTED, "the sequences' keys end at row %llu of the store's %llu", (ull)t->key_end,
+                    (ull)store->shape[0]);
+    *headroom = std::min(t->slack, store->shape[0] - t->key_end);
+    const uint64_t shape[2] = {t->queries, store->shape[1]};
+    Buffer* o;
+    MG_TRY(output_for(d, MG_F32, 2, shape, out, &o));
+    a->rows = nullptr;
+    a->dtype = MG_F32;
+    a->store = store->ptr;
+    a->store_dtype = MG_Q4;
+    a->queries = t->queries;
+    a->width = store->shape[1];
+    a->row_offset = 0;
+    *values = (float*)o->ptr;
+    return MG_OK;
+}
+
 mg_status attention_packed_plan(mg_device* h, const mg_buffer* qh, const mg_buffer* kh, const mg_buffer* vh,
                                 const mg_buffer* seqs, const mg_attention_params* pp, mg_buffer** out,
                                 k::PackedAttentionArgs* a, uint64_t* headroom) {
@@ -364,27 +392,12 @@ mg_status mg_kv_write_packed(mg_device* h, mg_buffer* store, const mg_buffer* ro
     return k::kv_write_packed(dev(h), a);
 }
 
-mg_status mg_kv_read_packed(mg_device* h, const mg_buffer* sh, const mg_buffer* sequences, mg_buffer** out) {
-    MG_TRY(device_check(h));
-    Device* d = dev(h);
-    MG_TRY(need(d, sh, "store"));
-    const Buffer* store = buf(sh);
-    if (store->dtype != MG_Q4) return fail(MG_DTYPE_UNSUPPORTED, "kv-read reads 4-bit stores, got %s", dtype_name(store->dtype));
-    k::KvPackedArgs a{};
-    const SequenceTable* t;
-    MG_TRY(need_table(d, sequences, &t, &a.table));
-    if (!t->writable) return fail(MG_SHAPE_UNSUPPORTED, "a sequence has fewer keys than rows to read");
-    if (t->key_end > store->shape[0])
-        return fail(MG_SHAPE_UNSUPPORTED, "the sequences' keys end at row %llu of the store's %llu", (ull)t->key_end,
-                    (ull)store->shape[0]);
-    const uint64_t shape[2] = {t->queries, store->shape[1]};
-    Buffer* o;
-    MG_TRY(output_for(d, MG_F32, 2, shape, out, &o));
-    a.store = store->ptr;
-    a.store_dtype = MG_Q4;
-    a.queries = t->queries;
-    a.width = store->shape[1];
-    return k::kv_read_packed(d, a, (float*)o->ptr);
+mg_status mg_kv_read_packed(mg_device* h, const mg_buffer* store, const mg_buffer* sequences, mg_buffer** out) {
+    k::KvPackedArgs a;
+    float* values;
+    uint64_t headroom;
+    MG_TRY(kv_read_packed_plan(h, store, sequences, out, &a, &values, &headroom));
+    return k::kv_read_packed(dev(h), a, values);
 }
 
 mg_status mg_attention_packed(mg_device* h, const mg_buffer* q, const mg_buffer* k, const mg_buffer* v,

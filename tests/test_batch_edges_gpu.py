@@ -280,3 +280,31 @@ def test_how_far_a_captured_step_may_advance(kernels, executor, mpc, queries, ke
         executor.run(node)
         executor.end_step_capture()
         assert executor.step_max_offset() == min(most, 100 - max(s + k for s, k in zip(starts, keys))), node
+
+
+def test_a_captured_read_back_follows_its_sequences(kernels, executor, mpc):
+    """kv-read-packed reads what kv-write-packed has just written, at every offset of a step."""
+    inv = mpc.KernelInvocation
+    ages, starts, total = [3, 60, 1], [0, 100, 200], 300
+    t = randn((total, 128), "f32", 245)
+    store = kernels.kv_store_q4(total, 2, 64)
+    kernels.kv_write(store, kernels.wrap_tensor(t), 0)
+    executor.adopt("store", store)
+    executor.adopt("seqs", kernels.sequences([1, 2, 1], ages, starts))
+    executor.write_zeroed_tensor("x", (4, 128))
+    nodes = [inv("kv-write-packed", ["store", "x", "seqs"], "store"), inv("kv-read-packed", ["store", "seqs"], "back")]
+    for node in nodes:
+        executor.run(node)
+    executor.begin_step_capture(["key_count"])
+    for node in nodes:
+        executor.run(node)
+    executor.end_step_capture()
+    assert executor.step_max_offset() == 40
+    x, back = np.empty((4, 128), np.float32), np.empty((4, 128), np.float32)
+    for offset in (0, 1, 7, 40):
+        x[:] = randn((4, 128), "f32", 246 + offset).cpu().numpy()
+        executor.replay_step_io({"x": x}, {"back": back}, offset=offset)
+        want = quantise64(torch.from_numpy(x).cuda())
+        assert torch.equal(torch.from_numpy(back).cuda().double(), want), offset
+        whole = torch.from_numpy(executor.read_tensor("store")).cuda().double()
+        assert torch.equal(whole[[s + m - n + i + offset for s, m, n in zip(starts, ages, [1, 2, 1]) for i in range(n)]], want)
