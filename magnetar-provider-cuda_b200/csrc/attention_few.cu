@@ -122,25 +122,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) attention_few_kernel(con
             for (int c = 0; c < C; c++) o[g][c] *= keep;
         }
         const float* v0 = values + (uint64_t)tile * 32 * ld;
-#pragma unroll 1
-        for (int j0 = 0; j0 < n; j0 += 8) {
+        auto add = [&](int j0, auto whole) {
             float v[8][C];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float* src = v0 + (uint64_t)min(j0 + j, n - 1) * ld;
                 if constexpr (C == 4) *reinterpret_cast<float4*>(v[j]) = __ldg(reinterpret_cast<const float4*>(src));
                 else *reinterpret_cast<float2*>(v[j]) = __ldg(reinterpret_cast<const float2*>(src));
+                // (a key past the last one: its weight of nothing would not keep an infinite value out)
+                if (!decltype(whole)::value && j0 + j >= n)
+#pragma unroll
+                    for (int c = 0; c < C; c++) v[j][c] = 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < 8; j++)
 #pragma unroll
                 for (int g = 0; g < G; g++) {
-                    // (a key past the last one has no weight)
                     const float w = __shfl_sync(0xffffffffu, weight[g], (j & 3) * 8 + (j0 + j) / 4);
 #pragma unroll
                     for (int c = 0; c < C; c++) o[g][c] = fmaf(w, v[j][c], o[g][c]);
                 }
-        }
+        };
+        int j0 = 0;
+#pragma unroll 1
+        for (; j0 + 8 <= n; j0 += 8) add(j0, std::true_type{});
+        if (j0 < n) add(j0, std::false_type{});
     }
 #pragma unroll
     for (int g = 0; g < G; g++) {

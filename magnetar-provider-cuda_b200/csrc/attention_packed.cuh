@@ -2,6 +2,8 @@
 // query row computed by one warp.
 #pragma once
 
+#include <type_traits>
+
 #include "sequences.cuh"
 
 namespace mg {
@@ -109,10 +111,10 @@ __device__ __forceinline__ void attention_keys(const k::PackedAttentionArgs& a, 
         const float keep = l > 0.0f ? l * alpha / l_new : 0.0f, weight = l_new != 0.0f ? e / l_new : 0.0f;
 #pragma unroll
         for (int i = 0; i < N; i++) o[i] *= keep;
-        // (addresses are bounded, not the loads: a conditional load is waited for at once; a lane past the last
-        // key has no weight, and a column past the last is not stored)
-#pragma unroll 1
-        for (int j0 = 0; j0 < keys; j0 += AHEAD) {
+        // (addresses are bounded, not the loads: a conditional load is waited for at once; a column past the last
+        // is not stored, and a key past the last counts as zeros, since its weight of nothing would not keep an
+        // infinite value out)
+        auto add = [&](int j0, auto whole) {
             float v[AHEAD][N];
 #pragma unroll
             for (int j = 0; j < AHEAD; j++)
@@ -122,9 +124,13 @@ __device__ __forceinline__ void attention_keys(const k::PackedAttentionArgs& a, 
             for (int j = 0; j < AHEAD; j++) {
                 const float w = __shfl_sync(0xffffffffu, weight, j0 + j);
 #pragma unroll
-                for (int i = 0; i < N; i++) o[i] = fmaf(w, v[j][i], o[i]);
+                for (int i = 0; i < N; i++) o[i] = fmaf(w, decltype(whole)::value || j0 + j < keys ? v[j][i] : 0.0f, o[i]);
             }
-        }
+        };
+        int j0 = 0;
+#pragma unroll 1
+        for (; j0 + AHEAD <= keys; j0 += AHEAD) add(j0, std::true_type{});
+        if (j0 < keys) add(j0, std::false_type{});
         m = m_new;
         l = l_new;
     }

@@ -308,3 +308,28 @@ def test_a_captured_read_back_follows_its_sequences(kernels, executor, mpc):
         assert torch.equal(torch.from_numpy(back).cuda().double(), want), offset
         whole = torch.from_numpy(executor.read_tensor("store")).cuda().double()
         assert torch.equal(whole[[s + m - n + i + offset for s, m, n in zip(starts, ages, [1, 2, 1]) for i in range(n)]], want)
+
+
+# ---------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (4, 2, 64), (3, 3, 80), (2, 1, 200), (2, 2, 300)])
+@pytest.mark.parametrize("queries,keys", [([1], [45]), ([1, 1], [3, 2001]), ([2], [1003]), ([5, 40], [5, 77]), ([1], [4999]), ([130], [130]), ([128], [128]), ([64], [256])])
+def test_infinite_values_that_a_query_sees(kernels, dtype, heads, kv, dim, queries, keys):
+    """An infinity in the last value row of a sequence is infinite for those who see it, and nothing to the others."""
+    q = randn((sum(queries), heads * dim), dtype, 251)
+    k, v = randn((sum(keys), kv * dim), dtype, 252), randn((sum(keys), kv * dim), dtype, 253)
+    v[-1, :2] = 0
+    finite = v.clone()
+    v[-1, 0], v[-1, 1] = math.inf, -math.inf
+    torch.cuda.synchronize()
+    seqs = kernels.sequences(queries, keys)
+    for causal, window in ((True, None), (True, 333), (False, None)):
+        got = to_torch(kernels, kernels.attention_packed(*(kernels.wrap_tensor(t) for t in (q, k, v)), seqs, heads, dim, kv_head_count=kv,
+                                                         causal=causal, window_size=window)).double()
+        want = attention64(q, k, finite, heads, kv, queries, keys, causal=causal, window=window)
+        first = sum(queries) - (1 if causal else queries[-1])
+        for h in range(heads // kv):
+            assert (got[first:, h * dim] == math.inf).all() and (got[first:, h * dim + 1] == -math.inf).all(), (causal, window)
+            got[first:, h * dim:h * dim + 2] = want[first:, h * dim:h * dim + 2]
+        assert torch.isfinite(got).all()
+        assert rel(got, want) <= ATTENTION_TOL[dtype], (causal, window)
