@@ -96,6 +96,8 @@ class PackedBatch:
         """Runs the prompts and keeps their keys and values; returns [tokens, 2 + 2 top]: of each token's
         successor in its prompt the log probability (NaN for the last), the entropy, the top alternatives."""
         ex, cfg, n = self.ex, self.cfg, [len(p) for p in prompts]
+        if not n or min(n) == 0:
+            raise ValueError(f"a batch needs prompts of at least one token each, got lengths {n}")
         if max(n) >= cfg.slot:
             raise ValueError(f"a prompt of {max(n)} tokens leaves no room in a slot of {cfg.slot}")
         self.lengths, self.steps = list(n), 0
