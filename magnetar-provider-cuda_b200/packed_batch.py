@@ -82,7 +82,7 @@ class PackedBatch:
     def __init__(self, ex: CudaExecutor, cfg: PackedBatchConfig, weights: Dict[str, np.ndarray]):
         if sum(cfg.sections) * 2 != cfg.head_dim:
             raise ValueError(f"sections {cfg.sections} do not make up the {cfg.head_dim // 2} pairs of a head")
-        self.ex, self.cfg, self.lengths, self.steps = ex, cfg, [], 0
+        self.ex, self.cfg, self.lengths, self.steps, self._replay = ex, cfg, [], 0, None
         for name in WEIGHTS:
             ex.write_weight_tensor(name, weights[name])
 
@@ -100,7 +100,7 @@ class PackedBatch:
             raise ValueError(f"a batch needs prompts of at least one token each, got lengths {n}")
         if max(n) >= cfg.slot:
             raise ValueError(f"a prompt of {max(n)} tokens leaves no room in a slot of {cfg.slot}")
-        self.lengths, self.steps = list(n), 0
+        self.lengths, self.steps, self._replay = list(n), 0, None
         ks = ex.kernels
         starts = [i * cfg.slot for i in range(len(n))]
         for name in ("key_store", "value_store"):
@@ -117,6 +117,8 @@ class PackedBatch:
 
     def capture(self) -> None:
         """Records a step.  (The rows that the recorded run writes are those that the first step writes again.)"""
+        if not self.lengths or self.steps:
+            raise RuntimeError("a step is captured after prefill and before the first step, whose rows the recorded run writes")
         ex, b = self.ex, len(self.lengths)
         self._ids, self._at = np.zeros(b, np.float32), np.zeros((b, len(self.cfg.sections)), np.float32)
         self._scores = np.empty((b, 2 + 2 * self.cfg.top), np.float32)
@@ -139,6 +141,8 @@ class PackedBatch:
     def step(self, ids: Sequence[int], positions=None) -> np.ndarray:
         """One more token of each sequence: [sequences, 2 + 2 top], the likeliest next tokens in the last
         ``top`` columns.  A step past the end of a slot is refused."""
+        if self._replay is None:
+            raise RuntimeError("a step needs capture() after the prefill")
         self._ids[:] = ids
         self._at[:] = self._positions(positions, [n + self.steps for n in self.lengths], [1] * len(self.lengths))
         self._replay(self.steps)
@@ -147,6 +151,8 @@ class PackedBatch:
 
     def generate(self, scores: np.ndarray, steps: int) -> List[List[int]]:
         """The likeliest continuation, from the scores of the prefill (or of the last step)."""
+        if self.cfg.top < 1:
+            raise ValueError("the likeliest tokens are among the alternatives: top is 0")
         top = scores[np.cumsum(self.lengths) - 1] if len(scores) != len(self.lengths) else scores
         tokens: List[List[int]] = [[] for _ in self.lengths]
         for _ in range(steps):
