@@ -319,7 +319,8 @@ mg_status mg_attention(mg_device* d, const mg_buffer* q, const mg_buffer* k, con
 /* ---------------------------------------------------------------------------------- */
 /* Batches of packed sequences -- no counterpart in the reference, which serves one     */
 /* sequence per call.  The rows of several sequences lie one after another in one        */
-/* buffer, with no padding; a table names each sequence's rows.                          */
+/* buffer, with no padding; a table names each sequence's rows.  Memory that a call       */
+/* writes shares none with its inputs (MG_INVALID_ARGUMENT), but mg_rope_axes' out.       */
 /* ---------------------------------------------------------------------------------- */
 
 /* The table of `count` sequences.  Sequence i owns the next query_counts[i] rows of a packed

@@ -8,6 +8,7 @@
 #include <cfloat>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <new>
 #include <numeric>
 
@@ -34,6 +35,21 @@ mg_status need_rows(const Buffer* b, const char* what, uint64_t* rows, uint64_t*
 
 mg_status need_float(const Buffer* b, const char* what) {
     if (!is_float(b->dtype)) return fail(MG_DTYPE_UNSUPPORTED, "%s cannot be %s", what, dtype_name(b->dtype));
+    return MG_OK;
+}
+
+// An offered output (or a store that is written) that shares memory with something the call reads: blocks of the
+// launch would read what others have already written.
+mg_status need_apart(const Buffer* written, std::initializer_list<const Buffer*> read) {
+    auto bytes = [](const Buffer* b) { return b->dtype == MG_Q4 ? q4_bytes(b->shape[0], b->shape[1]) : b->count * dtype_size(b->dtype); };
+    const uint8_t* w = (const uint8_t*)written->ptr;
+    for (const Buffer* b : read) {
+        if (!b || !bytes(b)) continue;
+        const uint8_t* r = (const uint8_t*)b->ptr;
+        if (w < r + bytes(b) && r < w + bytes(written))
+            return fail(MG_INVALID_ARGUMENT, "the memory that is written (%s) overlaps an input (%s)", shape_str(written).c_str(),
+                        shape_str(b).c_str());
+    }
     return MG_OK;
 }
 
@@ -184,6 +200,7 @@ mg_status kv_write_packed_plan(mg_device* h, mg_buffer* sh, const mg_buffer* rh,
     if (t->key_end > capacity)
         return fail(MG_SHAPE_UNSUPPORTED, "the sequences' keys end at row %llu of the store's %llu", (ull)t->key_end,
                     (ull)capacity);
+    MG_TRY(need_apart(store, {rows}));
     *headroom = std::min(t->write_slack, capacity - t->key_end);
     a->rows = rows->ptr;
     a->dtype = rows->dtype;
@@ -279,6 +296,7 @@ mg_status attention_packed_plan(mg_device* h, const mg_buffer* qh, const mg_buff
     const uint64_t shape[2] = {q_rows, heads * vdim};
     Buffer* o;
     MG_TRY(output_for(d, q->dtype, 2, shape, out, &o));
+    MG_TRY(need_apart(o, {q, kb, v}));
     a->q = q->ptr;
     a->k = kb->ptr;
     a->v = v->ptr;
@@ -473,6 +491,7 @@ mg_status mg_rope_axes(mg_device* h, const mg_buffer* xh, const mg_buffer* ph, c
                             (ull)p.sections[i]);
         Buffer* o;
         MG_TRY(output_for(d, x->dtype, 2, x->shape, out, &o));
+        MG_TRY(need_apart(o, {o->ptr == x->ptr ? nullptr : x, pos}));
         a.x = x->ptr;
         a.out = o->ptr;
         a.positions = (const float*)pos->ptr;
@@ -515,6 +534,7 @@ mg_status mg_token_logprobs(mg_device* h, const mg_buffer* lh, const mg_buffer* 
     const uint64_t shape[2] = {rows, 2 + 2 * (uint64_t)top};
     Buffer* o;
     MG_TRY(output_for(d, MG_F32, 2, shape, out, &o));
+    MG_TRY(need_apart(o, {l, t}));
     k::LogprobsArgs a;
     a.logits = l->ptr;
     a.dtype = l->dtype;

@@ -333,3 +333,32 @@ def test_infinite_values_that_a_query_sees(kernels, dtype, heads, kv, dim, queri
             got[first:, h * dim:h * dim + 2] = want[first:, h * dim:h * dim + 2]
         assert torch.isfinite(got).all()
         assert rel(got, want) <= ATTENTION_TOL[dtype], (causal, window)
+
+
+# ---------------------------------------------------------------------------- outputs over inputs
+def test_outputs_that_share_memory_with_inputs_are_refused(kernels, mpc):
+    """Blocks would read what others have written; rope in place is the one form that is in order."""
+    q, k = randn((8, 64), "f32", 261), randn((8, 64), "f32", 262)
+    whole = randn((20, 64), "f32", 263)
+    x, y = kernels.wrap_tensor(q), kernels.wrap_tensor(k)
+    seqs = kernels.sequences([8])
+    part = lambda first, rows: kernels.wrap_tensor(whole[first:first + rows])
+    logits, two = randn((6, 4), "f32", 264), randn((4, 2), "f32", 265)
+    lb, pb = kernels.wrap_tensor(logits), kernels.wrap_tensor(two)
+    calls = [lambda: kernels.attention_packed(x, y, y, seqs, 1, 64, out=x), lambda: kernels.attention_packed(x, y, y, seqs, 1, 64, out=y),
+             lambda: kernels.attention_packed(x, part(0, 8), part(8, 8), seqs, 1, 64, out=part(12, 8)),
+             lambda: kernels.kv_write_packed(part(0, 20), part(3, 8), seqs),
+             lambda: kernels.token_logprobs(lb, top=1, out=lb),
+             lambda: kernels.rope_axes(pb, pb, [1, 0], out=pb),
+             lambda: kernels.rope_axes(part(0, 8), kernels.zeros((8, 1)), [32], out=part(1, 8))]
+    before = [t.clone() for t in (q, k, whole, logits, two)]
+    for i, call in enumerate(calls):
+        with pytest.raises(mpc.CudaError) as e:
+            call()
+        assert e.value.code == "InvalidArgument", i
+    assert all(torch.equal(a, b) for a, b in zip(before, (q, k, whole, logits, two)))
+    # neighbours are apart
+    kernels.attention_packed(part(0, 4), part(4, 8), part(4, 8), kernels.sequences([4], [8]), 1, 64, out=part(12, 4))
+    kernels.kv_write_packed(part(0, 8), part(8, 8), seqs)
+    kernels.rope_axes(part(0, 8), kernels.zeros((8, 1)), [32], out=part(0, 8))
+    kernels.synchronize()
