@@ -388,12 +388,25 @@ __global__ void __launch_bounds__(kThreads, 1)
                     return true;
                 };
                 bool ok = load_k(0);
+                int k_loads = 1, v_loads = 0;
                 for (int j = 0; j < n_kv && ok; j++) {
-                    if (j + 1 < n_kv) ok = load_k(j + 1);
+                    if (j + 1 < n_kv) {
+                        ok = load_k(j + 1);
+                        k_loads += ok;
+                    }
                     const int s = j % S::kVStages;
                     if (ok && j >= S::kVStages) ok = mbar_wait(v_empty(s), (uint32_t)(j / S::kVStages - 1) & 1u);
-                    if (ok) load(base + S::kOffV + s * S::kStage, v_full(s), &map_v, &map_vlo, j);
+                    if (ok) {
+                        load(base + S::kOffV + s * S::kStage, v_full(s), &map_v, &map_vlo, j);
+                        v_loads++;
+                    }
                 }
+                // Whoever's wait may have run out, no copy is under way when the CTA leaves.
+                if constexpr (!kTwo) ok = mbar_wait(q_full, 0) && ok;
+                for (int j = max(0, k_loads - S::kKStages); j < k_loads; j++)
+                    ok = mbar_wait(k_full(j % S::kKStages), (uint32_t)(j / S::kKStages) & 1u) && ok;
+                for (int j = max(0, v_loads - S::kVStages); j < v_loads; j++)
+                    ok = mbar_wait(v_full(j % S::kVStages), (uint32_t)(j / S::kVStages) & 1u) && ok;
                 if (!ok) atomicExch(p.error, 1);
             }
             __syncwarp();

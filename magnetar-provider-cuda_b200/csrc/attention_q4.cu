@@ -217,6 +217,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
     uint8_t* ring = smem + warp * S::kRing;
     uint32_t filled = 0;  // tiles this warp has had (the phase of its ring)
     bool failed = false;
+    uint32_t missing = 0;  // the first tile that did not come
     T* out = (T*)p.a.out;
 
     // ---- row blocks, or the shares of them, one after another ---------------------------------------
@@ -251,7 +252,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
         const int see_hi = b_hi > b_lo ? (int)(((uint64_t)seq.k_start + (uint32_t)b_hi + 63) / 64) - tile_first : see_lo;
         const int tile0 = tile_first + max((int)first - kBlockCost, see_lo), tile1 = tile_first + min((int)(first + count) - kBlockCost, see_hi);
         const int tiles = tile1 - tile0;
-        const int mine = tiles > warp ? (tiles - warp + kWarps - 1) / kWarps : 0;  // tiles warp, warp + kWarps, ...
+        // tiles warp, warp + kWarps, ...; none after a wait has run out (the shares' arrivals still have to be counted)
+        const int mine = tiles > warp && !failed ? (tiles - warp + kWarps - 1) / kWarps : 0;
 
         const uint8_t* kbase = (const uint8_t*)p.a.k + ((uint64_t)(tile0 + warp) * columns + kvh * G) * kQ4Record;
         const uint8_t* vbase = (const uint8_t*)p.a.v + ((uint64_t)(tile0 + warp) * columns + kvh * G) * kQ4Record;
@@ -334,7 +336,10 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
             const uint32_t fill = filled + (uint32_t)i, s = fill % kStages;
             if (!mbar_wait(smem_u32(&bars[warp][s]), (fill / kStages) & 1u)) failed = true;
             failed = __any_sync(0xffffffffu, failed);
-            if (failed) break;
+            if (failed) {
+                missing = fill;
+                break;
+            }
             const uint8_t* kt = ring + s * 2 * S::kTile;
             const uint8_t* vt = kt + S::kTile;
             const int key0 = (int)((int64_t)(tile0 + warp + i * kWarps) * 64 - seq.k_start);  // of the tile, in the sequence (may be < 0)
@@ -667,7 +672,12 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? kPerSm : 2) attention_q4_k
         at += count;
         __syncthreads();  // the merge's shared memory becomes rings again
     }
-    if (failed && lane == 0) atomicExch(p.error, 1);
+    if (failed) {
+        // No copy is under way when the CTA leaves: one more wait for those it had asked for.
+        for (int i = 0; i < kStages; i++)
+            (void)mbar_wait(smem_u32(&bars[warp][(missing + i) % kStages]), ((missing + i) / kStages) & 1u);
+        if (lane == 0) atomicExch(p.error, 1);
+    }
 }
 
 template <typename T, int D, int NT>
