@@ -26,9 +26,9 @@ def _counts(values, like=None):
     values = [int(v) for v in values]
     if like is not None and len(values) != len(like):
         raise ValueError(f"{len(values)} counts for {len(like)} sequences")
-    if any(v < 0 for v in values):
-        raise ValueError("counts must not be negative")
-    return (ctypes.c_uint64 * max(1, len(values)))(*values) if values else (ctypes.c_uint64 * 0)()
+    if any(not 0 <= v < 2 ** 64 for v in values):
+        raise ValueError("counts must not be negative, nor pass 64 bits")
+    return (ctypes.c_uint64 * len(values))(*values)
 
 
 def _dtype_code(dtype) -> int:
@@ -250,14 +250,16 @@ class CudaKernels:
         """The table of a packed batch: sequence i owns the next ``query_counts[i]`` rows of the packed
         queries and ``key_counts[i]`` key rows (default: as many) from ``key_starts[i]`` on (default:
         one sequence after another)."""
-        q, k, s = _counts(query_counts), _counts(key_counts, query_counts), _counts(key_starts, query_counts)
+        q = _counts(query_counts)
+        k, s = _counts(key_counts, q), _counts(key_starts, q)
         out = ctypes.c_void_p()
         check(N.lib().mg_sequences_create(self._h, len(q), q, k, s, ctypes.byref(out)))
         return DeviceBuffer(out.value, self)
 
     def write_sequences(self, table, query_counts, key_counts=None, key_starts=None) -> DeviceBuffer:
         """New rows for a table of as many sequences, in stream order."""
-        q, k, s = _counts(query_counts), _counts(key_counts, query_counts), _counts(key_starts, query_counts)
+        q = _counts(query_counts)
+        k, s = _counts(key_counts, q), _counts(key_starts, q)
         check(N.lib().mg_sequences_write(table.handle, len(q), q, k, s))
         return table
 

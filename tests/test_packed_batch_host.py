@@ -1,4 +1,4 @@
-"""CPU: what PackedBatch refuses before it reaches the device."""
+"""CPU: what PackedBatch, and the tables of packed sequences, refuse before they reach the device."""
 import importlib
 
 import numpy as np
@@ -44,3 +44,14 @@ def test_continuations_need_an_alternative(mpc):
     batch.lengths = [2]
     with pytest.raises(ValueError, match="top is 0"):
         batch.generate(np.zeros((2, 2), np.float32), 1)
+
+
+def test_counts_of_a_table(mpc):
+    counts = importlib.import_module(mpc.__name__ + ".kernels")._counts
+    assert list(counts(range(3))) == [0, 1, 2] and list(counts([])) == [] and counts(None) is None
+    assert list(counts(np.array([4, 5]), counts(iter([1, 2])))) == [4, 5]  # as many as an iterator gave
+    for bad in ([-1], [2 ** 64], [2 ** 64 + 5]):
+        with pytest.raises(ValueError, match="64 bits"):
+            counts(bad)
+    with pytest.raises(ValueError, match="for 2 sequences"):
+        counts([1], counts([1, 1]))
