@@ -361,7 +361,10 @@ mg_status mg_kv_read_packed(mg_device* d, const mg_buffer* store, const mg_buffe
  * value_dimension 0 = head_dimension; window_size < 0 = none (requires causal); has_scale 0 =
  * 1/sqrt(D).  key_count is not used (the table has it) and must be negative.  A query that sees no
  * key gives zeros; keys outside a sequence or a mask are never weighed, whatever they hold.  Scores,
- * maxima and sums in f32.  Dimensions up to 512. */
+ * maxima and sums in f32.  Dimensions up to 512.  With heads of 64 or 128 and a sequence of more
+ * than two queries, f32 keys and values are copied as two 16-bit terms into a workspace of 8 bytes
+ * a (key, value) pair, for every key of every sequence with a captured step's largest advance (if
+ * memory has room for it). */
 mg_status mg_attention_packed(mg_device* d, const mg_buffer* q, const mg_buffer* k, const mg_buffer* v,
                               const mg_buffer* sequences, const mg_attention_params* params, mg_buffer** out);
 

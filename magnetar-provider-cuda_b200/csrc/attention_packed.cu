@@ -107,7 +107,15 @@ mg_status attention_q4(Device* d, const PackedAttentionArgs& a);
 mg_status attention_packed(Device* d, const PackedAttentionArgs& a) {
     if (a.queries == 0) return MG_OK;
     if (attention_few_eligible(a)) return attention_few(d, a);
-    if (attention_packed_tc_eligible(a)) return attention_packed_tc(d, a);
+    if (attention_packed_tc_eligible(a)) {
+        // The two-term copies of f32 keys and values hold a row for every key of every sequence (with a captured step's
+        // largest advance), 8 bytes a pair of values.  Where memory cannot hold them -- long rows that many sequences
+        // share -- the keys are read as they lie.
+        const mg_status s = attention_packed_tc(d, a);
+        if (s != MG_OUT_OF_DEVICE_MEMORY || a.dtype != MG_F32) return s;
+        clear_error();
+        return attention_few(d, a);
+    }
     if (attention_q4_eligible(a)) return attention_q4(d, a);
     return attention_packed_rows(d, a);
 }

@@ -335,6 +335,22 @@ def test_infinite_values_that_a_query_sees(kernels, dtype, heads, kv, dim, queri
         assert rel(got, want) <= ATTENTION_TOL[dtype], (causal, window)
 
 
+def test_more_shared_keys_than_memory_holds_copies_of(kernels):
+    """3000 sequences of three queries over the same 70000 rows: the copies that f32 prompts make of their keys would
+    take 215 GB."""
+    n, m, dim = 3000, 70000, 128
+    q, k, v = randn((3 * n, dim), "f32", 271), randn((m, dim), "f32", 272), randn((m, dim), "f32", 273)
+    seqs = kernels.sequences([3] * n, [m] * n, [0] * n)
+    got = to_torch(kernels, kernels.attention_packed(*(kernels.wrap_tensor(t) for t in (q, k, v)), seqs, 1, dim))
+    some = [0, 1, 1500, n - 1]
+    rows = torch.tensor([3 * i + j for i in some for j in range(3)], device="cuda")
+    assert rel(got[rows], attention64(q[rows], k, v, 1, 1, [3] * 4, [m] * 4, [0] * 4)) <= ATTENTION_TOL["f32"]
+    assert torch.isfinite(got).all()
+    prompt = kernels.sequences([100, 30])  # ordinary calls go on
+    got = to_torch(kernels, kernels.attention_packed(*(kernels.wrap_tensor(t[:130]) for t in (q, k, v)), prompt, 1, dim))
+    assert rel(got, attention64(q[:130], k, v, 1, 1, [100, 30], [100, 30])) <= ATTENTION_TOL["f32"]
+
+
 # ---------------------------------------------------------------------------- outputs over inputs
 def test_outputs_that_share_memory_with_inputs_are_refused(kernels, mpc):
     """Blocks would read what others have written; rope in place is the one form that is in order."""
