@@ -87,25 +87,6 @@ struct Params {
     uint32_t* again;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// The largest of three; NaN if one of them is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
-__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
 // Two values as a packed pair of the 16-bit type, the first in the low half.
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float a, float b) {

@@ -92,29 +92,10 @@ __device__ __forceinline__ uint32_t dequant(uint32_t word, int i, uint32_t magic
     return x;
 }
 
-// The largest of three; NaN if one of them is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-
 // The transpose of an 8 x 8 matrix of 16-bit values, two of a row in each lane's word.
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
-__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 

@@ -15,6 +15,8 @@
 namespace mg {
 namespace {
 
+using namespace sm100;
+
 constexpr int kThreads = 256;
 constexpr uint32_t kPerBlock = 4;  // threads of a block of 64 values, as q4_write_kernel takes it
 constexpr uint32_t kWriteBlocks = kThreads / kPerBlock, kReadBlocks = kThreads / 8;
@@ -43,17 +45,6 @@ struct Walk : Places<kStride> {
     }
 };
 
-__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-// The larger of two; NaN if one of them is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
 // A thread's sixteen values of a block, as they lie in memory.
 template <typename T, bool VEC>
 struct Sixteen {
@@ -120,7 +111,6 @@ struct Sixteen {
 // 28 us for 129 MB, 4.5 TB/s; half of the issue slots are taken.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads) q4_write_kernel(const k::KvPackedArgs a) {
-    using namespace sm100;
     constexpr int kPieces = kWriteBytes / (16 * (int)sizeof(T));
     pdl_enter();
     const uint32_t columns = (uint32_t)(a.width / kQ4Block);

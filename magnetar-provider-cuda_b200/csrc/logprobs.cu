@@ -43,23 +43,6 @@ struct LogprobsK {
     float floor;  // logits below it (excluded ones among them) are counted as it, see kNear and kFar
 };
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-// The larger of two; NaN if one of them is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
-}
-
 // Logits as they lie in memory: a 32-bit word of one or two, its larger and its values.
 template <typename T>
 struct Word;

@@ -141,7 +141,27 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  : "memory");
 }
 
-// ---- packed f32 pairs (fma / mul .rn.f32x2: each lane rounds as the scalar instruction) -------
+// ---- f32 --------------------------------------------------------------------------------------
+// 2^x to some 2^-22 of it; subnormal results are zero.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// The larger of two; NaN if one of them is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+// The largest of three; NaN if one of them is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// ---- packed f32 pairs (fma / mul / add .rn.f32x2: each lane rounds as the scalar instruction) --
 __device__ __forceinline__ uint64_t f2(float lo, float hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -153,6 +173,11 @@ __device__ __forceinline__ void f2fma(uint64_t& d, uint64_t a, uint64_t b) {
 __device__ __forceinline__ uint64_t f2mul(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ float2 f2split(uint64_t v) {
