@@ -5,6 +5,7 @@
 // keys up to and with that position, a window of w the last w of those.  A query that sees no key
 // gives zeros.
 #include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "attention_packed.cuh"
@@ -106,6 +107,14 @@ mg_status attention_q4(Device* d, const PackedAttentionArgs& a);
 
 mg_status attention_packed(Device* d, const PackedAttentionArgs& a) {
     if (a.queries == 0) return MG_OK;
+    // f32 queries take two bfloat16 terms per operand on the tensor cores (2-6e-6 of relative error against 64 bits) for
+    // 20 to 30 times the rate of f32 arithmetic (2-4e-7; 4 x 2048 tokens, 32 heads: 15.6 ms against 0.5), which a caller
+    // may have instead.
+    static const bool f32_throughout = [] {
+        const char* e = getenv("MAGNETAR_CUDA_PACKED_F32");
+        return e && atoi(e) != 0;
+    }();
+    if (f32_throughout && a.dtype == MG_F32) return attention_packed_tc_eligible(a) ? attention_few(d, a) : attention_packed_rows(d, a);
     if (attention_few_eligible(a)) return attention_few(d, a);
     if (attention_packed_tc_eligible(a)) {
         // The two-term copies of f32 keys and values hold a row for every key of every sequence (with a captured step's

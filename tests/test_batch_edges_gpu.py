@@ -351,6 +351,44 @@ def test_more_shared_keys_than_memory_holds_copies_of(kernels):
     assert rel(got, attention64(q[:130], k, v, 1, 1, [100, 30], [100, 30])) <= ATTENTION_TOL["f32"]
 
 
+_F32_CHILD = r"""
+import importlib, json, sys
+sys.path[:0] = [sys.argv[1], sys.argv[1] + "/tests"]
+import torch
+from test_batch_ops_gpu import attention64, quantise64, randn, rel, to_torch
+ks = importlib.import_module("magnetar-provider-cuda_b200").CudaKernels(0)
+out = []
+for heads, kv, dim, queries, keys in ((8, 2, 128, [300, 5, 41], [300, 700, 41]), (4, 4, 64, [130, 1], [130, 3000]), (3, 1, 64, [3, 4, 0], [999, 64, 7]),
+                                      (2, 1, 80, [50], [50])):
+    q, k, v = randn((sum(queries), heads * dim), "f32", 281), randn((sum(keys), kv * dim), "f32", 282), randn((sum(keys), kv * dim), "f32", 283)
+    seqs = ks.sequences(queries, keys)
+    for window in (None, 60):
+        got = to_torch(ks, ks.attention_packed(*(ks.wrap_tensor(t) for t in (q, k, v)), seqs, heads, dim, kv_head_count=kv, window_size=window))
+        out.append(rel(got, attention64(q, k, v, heads, kv, queries, keys, window=window)))
+        if dim % 64 == 0:
+            stores = [ks.kv_write(ks.kv_store_q4(sum(keys), kv, dim), ks.wrap_tensor(t), 0) for t in (k, v)]
+            got = to_torch(ks, ks.attention_packed(ks.wrap_tensor(q), *stores, seqs, heads, dim, kv_head_count=kv, window_size=window))
+            out.append(rel(got, attention64(q, quantise64(k), quantise64(v), heads, kv, queries, keys, window=window)))
+print(json.dumps(out))
+"""
+
+
+def test_f32_throughout_by_its_switch():
+    """Scores are sums of up to 128 products in four chains of f32, some 2^-21 off; weights, sums and means round by 2^-23:
+    2e-6 of the output bounds them, which two-term operands (2e-6 to 6e-6) do not reach."""
+    import json
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = lambda env: subprocess.run([sys.executable, "-c", _F32_CHILD, root], env=env, capture_output=True, text=True, timeout=300)
+    for value, bound in (("1", 2e-6), ("0", ATTENTION_TOL["f32"])):
+        res = run(dict(os.environ, MAGNETAR_CUDA_PACKED_F32=value))
+        assert res.returncode == 0, res.stderr[-2000:]
+        errors = json.loads(res.stdout.strip().splitlines()[-1])
+        assert len(errors) == 14 and max(errors) <= bound, errors
+
+
 # ---------------------------------------------------------------------------- outputs over inputs
 def test_outputs_that_share_memory_with_inputs_are_refused(kernels, mpc):
     """Blocks would read what others have written; rope in place is the one form that is in order."""
