@@ -5,7 +5,7 @@
 // (x - max) / temperature - log l once l is about c max itself: c max - r, which is no more than the rounding
 // of c max, is known exactly (one fused multiply-add), and so is every d up to the rounding of its own size.
 // The row is read once from memory (the top columns look at a part of it again, in the L2): 2 or 4
-// bytes a logit against one exponential and some six other instructions.
+// bytes a logit against one exponential and some ten other instructions.
 #include <algorithm>
 #include <cmath>
 
@@ -18,9 +18,9 @@ namespace {
 using namespace sm100;
 
 // Threads of an SM, of a block (where there are more rows than SMs), and 16-byte chunks of a thread in
-// flight.  8192 rows of 32000 bf16: 132 us, 4.0 TB/s, bound by instruction issue (two thirds of the slots,
-// half of the exponentials' unit); 1280 threads an SM 136, blocks of 128 threads 139 and of 512 172, 2 chunks
-// 138 (the 40 registers of 1536 threads just hold 4).
+// flight.  8192 rows of 32000 bf16: 134 to 139 us, 3.8 to 3.9 TB/s, bound by instruction issue (62 % of the
+// slots; 11.9 instructions a logit with 20 top columns).  Beside one such form of 132 us: 1280 threads an SM 136, blocks of 128
+// threads 139 and of 512 172, 2 chunks 138 (the 40 registers of 1536 threads just hold 4).
 constexpr int kPerSm = 1536, kBlock = 256, kBatch = 4;
 constexpr int kGroups = 64;  // at the most, of threads whose largest values are taken together: 32 or 64
 constexpr int kCandidates = 512;

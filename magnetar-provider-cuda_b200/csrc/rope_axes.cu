@@ -32,7 +32,7 @@ struct alignas(sizeof(T) * N == 16 ? 16 : alignof(T)) Vec {
 // the block's (row, pair)s go into shared memory, each computed once for all heads, then the values of
 // kItems heads are turned, N per access.  Streaming work: the bytes of x in and out bound it.  HALF: pairs are
 // (i, i + half) of a head, else (2i, 2i + 1); a thread owns both values of its pairs, so out may be x.
-// 32768 rows of 32 x 128 bf16: 84 to 88 us, 6.1 to 6.4 TB/s, nearly a copy's rate.  1, 2, 4 heads at a time take 90, 87 and
+// 32768 rows of 32 x 128 bf16: 84 to 90 us, 6.0 to 6.4 TB/s, nearly a copy's rate.  1, 2, 4 heads at a time take 90, 87 and
 // 84 (a turn is read from shared memory once for all of them); blocks of fewer rows, which leave threads
 // without a turn to compute, 111 to 132; turns laid out pair after pair (bank conflicts) 140.
 template <typename T, int N, bool HALF>
