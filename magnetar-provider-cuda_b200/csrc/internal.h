@@ -47,6 +47,7 @@ struct Device {
     cudaStream_t stream = nullptr;  // where work is enqueued
     cudaEvent_t order = nullptr;    // orders one stream behind another (made at its first use)
     cudaMemPool_t pool = nullptr;
+    size_t memory = SIZE_MAX;  // bytes the GPU has
     int sm_count = 148;
     int sm_major = 10, sm_minor = 0;
     std::atomic<uint64_t> uploads{0}, downloads{0}, launches{0};

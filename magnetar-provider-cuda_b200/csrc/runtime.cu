@@ -84,7 +84,9 @@ mg_status device_alloc(Device* d, size_t bytes, void** ptr) {
     *ptr = nullptr;
     if (bytes == 0) bytes = 16;  // a device buffer is never empty (src/kernels.rs:4454-4455)
     cudaError_t e;
-    if (d->capturing) {
+    if (bytes > d->memory) {  // (a pool would take all that there is before it found out)
+        e = cudaErrorMemoryAllocation;
+    } else if (d->capturing) {
         e = cudaMalloc(ptr, bytes);
         if (e == cudaSuccess) {
             std::lock_guard<std::mutex> g(d->mem_lock);
@@ -97,6 +99,8 @@ mg_status device_alloc(Device* d, size_t bytes, void** ptr) {
     if (e != cudaSuccess) {
         cudaGetLastError();
         *ptr = nullptr;
+        // What the pool took for the block it could not complete goes back; it keeps free blocks otherwise.
+        if (e == cudaErrorMemoryAllocation && !d->capturing) cudaMemPoolTrimTo(d->pool, 0);
         return fail(e == cudaErrorMemoryAllocation ? MG_OUT_OF_DEVICE_MEMORY : MG_DRIVER_FAILED,
                     "allocating %zu bytes on cuda:%d: %s", bytes, d->ordinal, cudaGetErrorString(e));
     }
@@ -403,6 +407,7 @@ mg_status mg_device_open(int ordinal, mg_device** out) {
     if (!d) return fail(MG_EXECUTION_FAILED, "host allocation failed");
     d->ordinal = ordinal;
     d->sm_count = prop.multiProcessorCount;
+    d->memory = prop.totalGlobalMem;
     d->sm_major = prop.major;
     d->sm_minor = prop.minor;
     const char* pdl = getenv("MAGNETAR_CUDA_PDL");

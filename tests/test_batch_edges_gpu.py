@@ -389,6 +389,19 @@ def test_f32_throughout_by_its_switch():
         assert len(errors) == 14 and max(errors) <= bound, errors
 
 
+def test_a_refused_allocation_leaves_the_memory_free(kernels, mpc):
+    """More than the GPU has, and all that it has (of which the process itself has a part): refused, and nothing is kept of it."""
+    torch.cuda.empty_cache()
+    kernels.synchronize()
+    before = kernels.info()
+    for size in (before["total_bytes"] + 2 ** 32, before["total_bytes"] - 2 ** 20):
+        with pytest.raises(mpc.CudaError) as e:
+            kernels.empty((size // 4,))
+        assert e.value.code == "OutOfDeviceMemory"
+        assert kernels.info()["free_bytes"] >= before["free_bytes"] - 2 ** 28
+    assert not kernels.download(kernels.zeros((1000,))).any()
+
+
 # ---------------------------------------------------------------------------- outputs over inputs
 def test_outputs_that_share_memory_with_inputs_are_refused(kernels, mpc):
     """Blocks would read what others have written; rope in place is the one form that is in order."""
