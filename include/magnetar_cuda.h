@@ -364,7 +364,8 @@ mg_status mg_kv_read_packed(mg_device* d, const mg_buffer* store, const mg_buffe
  * maxima and sums in f32.  Dimensions up to 512.  With heads of 64 or 128 and a sequence of more
  * than two queries, f32 keys and values are copied as two 16-bit terms into a workspace of 8 bytes
  * a (key, value) pair, for every key of every sequence with a captured step's largest advance (if
- * memory has room for it). */
+ * memory has room for it).  Where a row has more than 2048 keys (f32; else 16384), another holds its
+ * head's sums, 4 * D bytes a query and head in whole blocks of 256 rows. */
 mg_status mg_attention_packed(mg_device* d, const mg_buffer* q, const mg_buffer* k, const mg_buffer* v,
                               const mg_buffer* sequences, const mg_attention_params* params, mg_buffer** out);
 

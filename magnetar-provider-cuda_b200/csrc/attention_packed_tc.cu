@@ -15,6 +15,11 @@
 // The offset (2^40 for weights with f32's exponent range) keeps O below the largest |v|
 // however many keys are summed, so large finite values cannot overflow the sum.
 //
+// The tensor cores add into their accumulators by cutting digits off, not by rounding, so that every sum of 16 products
+// takes an output some 2^-24 of itself towards zero: 5e-9 a key, 2e-4 after 32768 keys.  After kKeysSummed keys O is
+// therefore added to sums in memory, in f32, and starts again from zero: 1024 f32 queries over 131072 keys are 1e-5 off
+// instead of 8e-4, for 3 to 5 % of the time of long rows (one f32 prompt of 8192 tokens, 32 heads, 1335 -> 1399 us).
+//
 // f32 operands are two bfloat16 terms each, hi + lo, and three products: lo hi + hi lo + hi hi; K and V
 // are split by a pass of their own into a workspace of the sequences' rows one after another, a query
 // row by the thread that owns it.
@@ -60,6 +65,10 @@ struct Shape {
     static constexpr int kKeys = kTerms == 2 ? 64 : 128;   // keys of a tile
     static constexpr int kScores = 128 / kKeys;            // score buffers of a query tile
     static constexpr int kParts = kKeys / 32;              // weights of a tile are handed over 32 keys at a time
+    // Keys that O sums in tensor memory before it is taken out: up to 1e-5 of it are lost, for the 16-bit types 8e-5, a
+    // third of f16's own rounding (a bfloat16 prompt of 32768 tokens 7.08 -> 7.27 ms).
+    static constexpr int kKeysSummed = kTerms == 2 ? 2048 : 16384;
+    static constexpr int kTilesSummed = kKeysSummed / kKeys;
     static constexpr int kQAtom = kRows * 128;             // [128 rows][64 columns], 128-byte swizzle
     static constexpr int kQTerm = (D / 64) * kQAtom;
     static constexpr int kQTile = kTerms * kQTerm;
@@ -88,6 +97,9 @@ struct Params {
     float* means;
     float2* stats;
     uint32_t* again;
+    // O taken out of tensor memory (where a row has more than kKeysSummed keys): column c of the row of warp
+    // 4 + w, lane l of CTA i at ((i * 8 + w) * (D + 1) + c) * 32 + l, and its reference as column D.
+    float* summed;
 };
 
 // Two values as a packed pair of the 16-bit type, the first in the low half.
@@ -458,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     const int kk = 2 * part + k2;
                                     const uint64_t v = dv + (uint64_t)((kk * 2048) >> 4);
                                     const uint32_t pa = tP + (uint32_t)kk * 8;
-                                    const uint32_t acc = (j > 0 || kk > 0) ? 1u : 0u;
+                                    const uint32_t acc = (j % S::kTilesSummed > 0 || kk > 0) ? 1u : 0u;
                                     if constexpr (kTwo) {
                                         mma_ts(lead, tO, pa + KV / 2, v, idesc_o, acc);
                                         mma_ts(lead, tO, pa, v + (uint64_t)(S::kTerm >> 4), idesc_o, 1u);
@@ -590,105 +602,140 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tO = lane_base + S::kColO + (uint32_t)(D * t);
         const int n = n_t[t];
         float m = kNegInf, l = 0.0f;
+        auto summed = [&]() { return p.summed + ((uint64_t)blockIdx.x * 8 + (uint32_t)(warp - 4)) * ((D + 1) * 32) + lane; };
+        // 2^(their reference - now's), of the values there
+        auto summed_by = [&](const float* at, float now) {
+            const float then = __ldcg(at + D * 32);
+            return then == now ? 1.0f : ex2(then - now);
+        };
         bool failed = false;
-        for (int j = 0; j < n; j++) {
-            failed = !mbar_wait(s_full(t, j % S::kScores), (uint32_t)(j / S::kScores) & 1u);
-            failed = __any_sync(0xffffffffu, failed);
-            if (failed) break;
-            tc_fence_after();
-            const uint32_t tS = lane_base + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
-            float s[KV];
-            const int key0 = kv0 + j * KV;
-            const bool part_seen = key0 < row_lo || key0 + KV > row_hi;
-#pragma unroll
-            for (int c = 0; c < KV; c += 32) tmem_ld32(tS + (uint32_t)c, s + c);
-            tc_wait_ld();
-            if (part_seen) {
-                const int lo = row_lo - key0, hi = row_hi - key0;
-#pragma unroll
-                for (int c = 0; c < KV; c++) s[c] = c >= lo && c < hi ? s[c] : kNegInf;
-            }
-            // the row's maximum of the raw scores (sc > 0 keeps their order), in log2 units
-            float mx[4];
-#pragma unroll
-            for (int g = 0; g < 4; g++) mx[g] = max3(s[g], s[g + 4], s[g + 8]);
-#pragma unroll
-            for (int c = 12; c + 4 < KV; c += 8)
-#pragma unroll
-                for (int g = 0; g < 4; g++) mx[g] = max3(mx[g], s[c + g], s[c + 4 + g]);
-#pragma unroll
-            for (int g = 0; g < 4; g++) mx[g] = max3(mx[g], s[KV - 4 + g], s[KV - 4 + g]);
-            const float tmax = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sc;
-            // the reference moves only when this tile's maximum passes it by more than kLazy; scores that are
-            // NaN or +inf make it NaN, and with it all of the row
-            bool move = tmax != kNegInf && !(tmax <= m + kLazy);
-            float f = 1.0f;
-            if (move) {
-                f = m == kNegInf ? 0.0f : ex2(m - tmax);
-                move = m != kNegInf;  // an O that holds only zero weights needs no rescale
-                m = fmaf(tmax, 0.0f, tmax);
-                l *= f;
-            }
-            if (j > 0 && __any_sync(0xffffffffu, move)) {
-                // O *= f, once P V(j - 1) has completed
-                failed = !mbar_wait(pv_done(t, (j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u);
+        for (int j = 0; j < n && !failed;) {
+            for (const int stop = min(n, j + S::kTilesSummed); j < stop; j++) {
+                failed = !mbar_wait(s_full(t, j % S::kScores), (uint32_t)(j / S::kScores) & 1u);
                 failed = __any_sync(0xffffffffu, failed);
                 if (failed) break;
                 tc_fence_after();
-                const float g = move ? f : 1.0f;
+                const uint32_t tS = lane_base + 128u * (uint32_t)t + (uint32_t)(j % S::kScores) * KV;
+                float s[KV];
+                const int key0 = kv0 + j * KV;
+                const bool part_seen = key0 < row_lo || key0 + KV > row_hi;
+#pragma unroll
+                for (int c = 0; c < KV; c += 32) tmem_ld32(tS + (uint32_t)c, s + c);
+                tc_wait_ld();
+                if (part_seen) {
+                    const int lo = row_lo - key0, hi = row_hi - key0;
+#pragma unroll
+                    for (int c = 0; c < KV; c++) s[c] = c >= lo && c < hi ? s[c] : kNegInf;
+                }
+                // the row's maximum of the raw scores (sc > 0 keeps their order), in log2 units
+                float mx[4];
+#pragma unroll
+                for (int g = 0; g < 4; g++) mx[g] = max3(s[g], s[g + 4], s[g + 8]);
+#pragma unroll
+                for (int c = 12; c + 4 < KV; c += 8)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) mx[g] = max3(mx[g], s[c + g], s[c + 4 + g]);
+#pragma unroll
+                for (int g = 0; g < 4; g++) mx[g] = max3(mx[g], s[KV - 4 + g], s[KV - 4 + g]);
+                const float tmax = max3(max3(mx[0], mx[1], mx[2]), mx[3], mx[3]) * sc;
+                // the reference moves only when this tile's maximum passes it by more than kLazy; scores that are
+                // NaN or +inf make it NaN, and with it all of the row
+                bool move = tmax != kNegInf && !(tmax <= m + kLazy);
+                float f = 1.0f;
+                if (move) {
+                    f = m == kNegInf ? 0.0f : ex2(m - tmax);
+                    move = m != kNegInf;  // an O that holds only zero weights needs no rescale
+                    m = fmaf(tmax, 0.0f, tmax);
+                    l *= f;
+                }
+                if (j > 0 && __any_sync(0xffffffffu, move)) {
+                    // O *= f, once P V(j - 1) has completed
+                    failed = !mbar_wait(pv_done(t, (j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u);
+                    failed = __any_sync(0xffffffffu, failed);
+                    if (failed) break;
+                    tc_fence_after();
+                    const float g = move ? f : 1.0f;
 #pragma unroll 1
-                for (int c = 0; c < D; c += 16) {
-                    float o[16];
-                    tmem_ld16(tO + (uint32_t)c, o);
-                    tc_wait_ld();
-                    uint32_t u[16];
+                    for (int c = 0; c < D; c += 16) {
+                        float o[16];
+                        tmem_ld16(tO + (uint32_t)c, o);
+                        tc_wait_ld();
+                        uint32_t u[16];
 #pragma unroll
-                    for (int e = 0; e < 16; e++) u[e] = __float_as_uint(o[e] * g);
-                    tmem_st16(tO + (uint32_t)c, u);
+                        for (int e = 0; e < 16; e++) u[e] = __float_as_uint(o[e] * g);
+                        tmem_st16(tO + (uint32_t)c, u);
+                    }
+                    tc_wait_st();
                 }
-                tc_wait_st();
-            }
-            // (no key seen yet: every score is -inf, and weights 2^(-inf) are 0)
-            const float ref = m == kNegInf ? 0.0f : -(m + kOffset);
-            const uint64_t sc2 = f2(sc, sc), ref2 = f2(ref, ref);
-            uint64_t sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
-            auto hand_over = [&](int part) {
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive_warp(p_full(t, j % S::kScores, part));
-            };
+                // (no key seen yet: every score is -inf, and weights 2^(-inf) are 0)
+                const float ref = m == kNegInf ? 0.0f : -(m + kOffset);
+                const uint64_t sc2 = f2(sc, sc), ref2 = f2(ref, ref);
+                uint64_t sum[2] = {f2(0.0f, 0.0f), f2(0.0f, 0.0f)};
+                auto hand_over = [&](int part) {
+                    tc_wait_st();
+                    tc_fence_before();
+                    mbar_arrive_warp(p_full(t, j % S::kScores, part));
+                };
 #pragma unroll
-            for (int part = 0; part < S::kParts; part++) {
-                // 32 weights, over the scores just read
-                uint32_t h[16];
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int c = part * 32 + 2 * e;
-                    uint64_t x = ref2;
-                    f2fma(x, f2(s[c], s[c + 1]), sc2);
-                    const float2 y = f2split(x);
-                    s[c] = ex2(y.x);
-                    s[c + 1] = ex2(y.y);
-                    sum[e & 1] = f2add(sum[e & 1], f2(s[c], s[c + 1]));
-                    h[e] = pack16<T>(s[c], s[c + 1]);
-                }
-                if (part > 0) hand_over(part - 1);  // (the stores before it have had this part's time)
-                tmem_st16(tS + (uint32_t)(part * 16), h);
-                if constexpr (kTwo) {
-                    uint32_t lo[16];
+                for (int part = 0; part < S::kParts; part++) {
+                    // 32 weights, over the scores just read
+                    uint32_t h[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
                         const int c = part * 32 + 2 * e;
-                        lo[e] = pack16<T>(s[c] - __uint_as_float(h[e] << 16), s[c + 1] - __uint_as_float(h[e] & 0xffff0000u));
+                        uint64_t x = ref2;
+                        f2fma(x, f2(s[c], s[c + 1]), sc2);
+                        const float2 y = f2split(x);
+                        s[c] = ex2(y.x);
+                        s[c + 1] = ex2(y.y);
+                        sum[e & 1] = f2add(sum[e & 1], f2(s[c], s[c + 1]));
+                        h[e] = pack16<T>(s[c], s[c + 1]);
                     }
-                    tmem_st16(tS + (uint32_t)(KV / 2 + part * 16), lo);
+                    if (part > 0) hand_over(part - 1);  // (the stores before it have had this part's time)
+                    tmem_st16(tS + (uint32_t)(part * 16), h);
+                    if constexpr (kTwo) {
+                        uint32_t lo[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const int c = part * 32 + 2 * e;
+                            lo[e] = pack16<T>(s[c] - __uint_as_float(h[e] << 16), s[c + 1] - __uint_as_float(h[e] & 0xffff0000u));
+                        }
+                        tmem_st16(tS + (uint32_t)(KV / 2 + part * 16), lo);
+                    }
                 }
+                hand_over(S::kParts - 1);
+                const float2 u = f2split(f2add(sum[0], sum[1]));
+                l += u.x + u.y;
             }
-            hand_over(S::kParts - 1);
-            const float2 u = f2split(f2add(sum[0], sum[1]));
-            l += u.x + u.y;
+            if (failed || j >= n) break;
+            // O to memory; the next P V starts from zero
+            failed = !mbar_wait(pv_done(t, (j - 1) & 1), (uint32_t)((j - 1) >> 1) & 1u);
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+            tc_fence_after();
+            float* at = summed();
+            const float by = j > S::kTilesSummed ? summed_by(at, m) : 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                float o[32], before[32];
+                // (loaded the first time too, and not used: a conditional load is waited for at once)
+#pragma unroll
+                for (int e = 0; e < 32; e++) before[e] = __ldcg(at + (c + e) * 32);
+                tmem_ld32(tO + (uint32_t)c, o);
+                tc_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; e++) __stcg(at + (c + e) * 32, j > S::kTilesSummed ? fmaf(before[e], by, o[e]) : o[e]);
+            }
+            __stcg(at + D * 32, m);
         }
         // ---- the output row: O / l ---------------------------------------------------------------
+        auto whole = [&](int c, float* o) {  // with what was taken out
+            if (n <= S::kTilesSummed) return;
+            const float* at = summed();
+            const float by = summed_by(at, m);
+#pragma unroll
+            for (int e = 0; e < 32; e++) o[e] = fmaf(__ldcg(at + (c + e) * 32), by, o[e]);
+        };
         bool have = false;
         if (n > 0 && !failed) {
             failed = !mbar_wait(pv_done(t, (n - 1) & 1), (uint32_t)((n - 1) >> 1) & 1u);
@@ -710,6 +757,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (have) {
                     tmem_ld32(tO + (uint32_t)c, o);  // (by the whole warp)
                     tc_wait_ld();
+                    whole(c, o);
                 }
                 if (live) {
                     float4* dst = reinterpret_cast<float4*>(p.means + ((uint64_t)blockIdx.x * p.live + row) * D + c);
@@ -737,6 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float o[32];
                 tmem_ld32(tO + (uint32_t)c, o);
                 tc_wait_ld();
+                whole(c, o);
 #pragma unroll
                 for (int e = 0; e < 32; e += N) {
                     uint4 v;
@@ -893,6 +942,7 @@ mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
     p.means = nullptr;
     p.stats = nullptr;
     p.again = nullptr;
+    p.summed = nullptr;
     uint64_t items = 0;
     for (const SeqRow& r : a.host->rows) items += (r.q_count + p.tokens - 1) / p.tokens;
     if (items * p.groups > 0x7fffffffull) return fail(MG_SHAPE_UNSUPPORTED, "attention launch size overflows");
@@ -936,6 +986,10 @@ mg_status launch(Device* d, const k::PackedAttentionArgs& a) {
     uint64_t longest = 0;
     for (const SeqRow& r : a.host->rows) longest = std::max<uint64_t>(longest, r.k_count + a.max_step);
     const uint64_t parts = ctas ? std::min<uint64_t>((uint64_t)d->sm_count / ctas, longest / kPartKeys) : 0;
+    // A row sees at most `span` keys, a CTA's tiles as many and its tokens' more.
+    const uint64_t span = a.causal && a.window >= 0 ? std::min(longest, (uint64_t)a.window + p.tokens) : longest;
+    if (span > (uint64_t)S::kKeysSummed)
+        MG_TRY(scratch(d, 10, ctas * std::max<uint64_t>(1, parts) * 2 * kRows * (D + 1) * sizeof(float), (void**)&p.summed));
     if (parts < 2) {
         enqueue(d, attention_packed_tc_kernel<T, D, false>, (unsigned)ctas, kThreads, S::kSmem, maps[0], maps[1], maps[2], maps[3], maps[4], p);
         return launched(d, "packed attention launch");

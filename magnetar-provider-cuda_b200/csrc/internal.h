@@ -39,7 +39,7 @@ void clear_error();
     } while (0)
 
 // ---- device ----------------------------------------------------------------------------
-constexpr int kScratchSlots = 10;
+constexpr int kScratchSlots = 11;
 
 struct Device {
     int ordinal = 0;

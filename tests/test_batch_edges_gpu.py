@@ -351,6 +351,58 @@ def test_more_shared_keys_than_memory_holds_copies_of(kernels):
     assert rel(got, attention64(q[:130], k, v, 1, 1, [100, 30], [100, 30])) <= ATTENTION_TOL["f32"]
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv,dim,queries,keys,window", [
+    (40, 40, 64, [300], [20000], None),             # a CTA has all keys of its rows
+    (24, 8, 128, [600, 1, 400], [17000, 9, 18500], None),
+    (40, 40, 64, [700], [24000], 18000),
+    (8, 8, 128, [8], [70000], None),                # the keys are split, and a part is still long
+    (32, 8, 128, [4, 2], [50000, 300], 45000),
+])
+def test_sums_over_many_keys(kernels, dtype, heads, kv, dim, queries, keys, window):
+    """Tens of thousands of keys, values that do not cancel (sums on the tensor cores lose a little of themselves with
+    every addition), later keys with ever higher scores (what has been summed is scaled down)."""
+    q = randn((sum(queries), heads * dim), dtype, 291)
+    k, v = randn((sum(keys), kv * dim), dtype, 292), randn((sum(keys), kv * dim), "f32", 293)
+    v = (v + 1).to(DT[dtype])
+    some = torch.cat([torch.arange(b - n, b, max(1, n // 12), device="cuda") for n, b in zip(queries, np.cumsum(queries).tolist())])
+    for rising in (False, True):
+        if rising:
+            k = (k.float() * torch.linspace(0.2, 2.5, sum(keys), device="cuda")[:, None]).to(DT[dtype])
+        torch.cuda.synchronize()
+        got = to_torch(kernels, kernels.attention_packed(*(kernels.wrap_tensor(t) for t in (q, k, v)), kernels.sequences(queries, keys), heads, dim,
+                                                         kv_head_count=kv, window_size=window))
+        assert torch.isfinite(got).all()
+        at_q = at_k = 0
+        for n, m in zip(queries, keys):  # a row at a time: it is the last of its own keys
+            rows = [int(r) for r in some if at_q <= r < at_q + n]
+            for r in rows:
+                seen = m - n + (r - at_q) + 1
+                want = attention64(q[r:r + 1], k[at_k:at_k + seen], v[at_k:at_k + seen], heads, kv, [1], [seen], window=window)
+                assert rel(got[r], want[0]) <= ATTENTION_TOL[dtype], (rising, r)
+            at_q, at_k = at_q + n, at_k + m
+
+
+def test_sums_over_many_keys_in_a_captured_step(kernels, executor, mpc):
+    """A step captured over a few keys, replayed where they are many."""
+    inv = mpc.KernelInvocation
+    heads, dim, slot, n = 8, 64, 40000, 4
+    q, k, v = randn((n, heads * dim), "f32", 295), randn((slot, heads * dim), "f32", 296), randn((slot, heads * dim), "f32", 297) + 1
+    torch.cuda.synchronize()
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        executor.write_tensor(name, t.cpu().numpy())
+    executor.adopt("seqs", kernels.sequences([n], [10], [0]))
+    node = inv("attention-packed", ["q", "k", "v", "seqs"], "out", {"head_count": heads, "head_dimension": dim, "causal": True})
+    executor.run(node)
+    executor.begin_step_capture(["key_count"])
+    executor.run(node)
+    executor.end_step_capture()
+    for offset in (0, 2040, 2300, 39990):
+        executor.replay_step(offset=offset)
+        got = torch.from_numpy(executor.read_tensor("out")).cuda()
+        assert rel(got, attention64(q, k, v, heads, heads, [n], [10 + offset])) <= ATTENTION_TOL["f32"], offset
+
+
 _F32_CHILD = r"""
 import importlib, json, sys
 sys.path[:0] = [sys.argv[1], sys.argv[1] + "/tests"]
