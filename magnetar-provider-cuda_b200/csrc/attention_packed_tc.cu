@@ -35,7 +35,7 @@
 // which their own rounding is 1.6e-3, and two terms of f32 operands 6e-6, where f32 arithmetic has 4e-7.
 //
 // Causal, heads of 128: ten prompts of 1 to 8192 tokens, 32 heads over 8, bfloat16, 719 to 739 us, 1.02 to 1.05
-// PFLOP/s, the tensor pipe busy for 59 % (the chain scores, softmax, product of two tiles sets the pace); 4 x 2048 tokens,
+// PFLOP/s, the tensor pipe busy for 58 % (the chain scores, softmax, product of two tiles sets the pace); 4 x 2048 tokens,
 // 32 heads, f32, 557 to 569 us with the split, 242 to 247 TFLOP/s, three times that on the tensor cores.
 #include <cuda.h>
 #include <cudaTypedefs.h>

@@ -29,7 +29,7 @@
 // (One bfloat16 term for the weights is what their products' rate allows: outputs are 2.3e-3 off, of which their own
 // rounding is 1.7e-3; two terms leave 3.8e-6 where f32 arithmetic has 5e-7.)
 //
-// One query each, 32 heads over 8 of 128: 16 sequences, 15 of 32768 keys and one of 131071, bfloat16, 149 to 156 us,
+// One query each, 32 heads over 8 of 128: 16 sequences, 15 of 32768 keys and one of 131071, bfloat16, 147 to 156 us,
 // 4.4 to 4.6 TB/s of the store (half of the ALU's slots); 32 sequences of some 100 to 16000 keys, f32, 41 us.
 #include <algorithm>
 #include <type_traits>
